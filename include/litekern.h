@@ -46,6 +46,12 @@ extern "C" {
 #define LK_DTYPE_F16 1
 #define LK_DTYPE_BF16 2
 
+/* How a KV cache holds its rows: as the 16-bit element type of the query, or
+ * in 8 bits with one fp32 scale per row (lk_store_kv_q8). */
+#define LK_KV_16BIT 0
+#define LK_KV_INT8 1
+#define LK_KV_E4M3 2
+
 /* Bits the kernels OR into a caller-provided device status word. */
 #define LK_STATUS_SLOT_OOB 1       /* slot_mapping entry >= num_slots or < -1 */
 #define LK_STATUS_BLOCK_OOB 2      /* block table entry outside [0, num_blocks) */
@@ -75,6 +81,47 @@ int lk_store_kv(const void* key, const void* value, void* k_cache, void* v_cache
                 int32_t num_kv_heads, int32_t head_dim,
                 int64_t key_token_stride, int64_t value_token_stride,
                 int64_t num_slots, int32_t dtype, int32_t* status, void* stream);
+
+/*
+ * 8-bit KV-cache store: lk_store_kv with each (token, KV head) row quantised
+ * as it is written. No counterpart in the reference (its cache has the
+ * model's type). For a row x[0..D), with M = 127 (LK_KV_INT8) or 448
+ * (LK_KV_E4M3):
+ *   a = max(max |x|, 2^-100),  scale = RN32(a / M),  r = RN32(M / a)
+ *   int8: q = rint(x r) of the exact product, ties to even
+ *   e4m3: q = RN_e4m3(RN32(x r))
+ * A row with an infinity or a NaN is stored as zeros with scale NaN. k_data /
+ * v_data: bytes [num_blocks, block_size, H_kv, D], 16-byte aligned; k_scale /
+ * v_scale: fp32 [num_blocks, H_kv, block_size]. key / value: F16 or BF16,
+ * [num_tokens, H_kv, D] with head stride D, unit element stride and a token
+ * stride in elements. D is 64 or 128. Slots as for lk_store_kv: -1 is
+ * skipped, others outside the cache are skipped and flagged; of two tokens
+ * with the same slot it is unspecified which part of which is kept.
+ */
+int lk_store_kv_q8(const void* key, const void* value, void* k_data, float* k_scale,
+                   void* v_data, float* v_scale, const int64_t* slot_mapping,
+                   int32_t num_tokens, int32_t H_kv, int32_t D,
+                   int64_t key_token_stride, int64_t value_token_stride,
+                   int64_t num_blocks, int32_t block_size, int32_t dtype, int32_t kv_format,
+                   int32_t* status, void* stream);
+
+/*
+ * Read an 8-bit cache back: row cu_rows[b] + p of key_out / value_out
+ * ([num_rows, H_kv, D] contiguous, F32, F16 or BF16, 16-byte aligned) is
+ * scale * q of position p of sequence b, rounded once, for
+ * p < context_lens[b], and zero for the sequence's rows past its context.
+ * cu_rows: int32 [num_seqs + 1], not decreasing; rows before cu_rows[0] or
+ * from cu_rows[num_seqs] on are left as they were. A context longer than the
+ * table is flagged LK_STATUS_CTX_OOB and its rows past the table are zero; a
+ * block id outside the cache gives zero rows and LK_STATUS_BLOCK_OOB.
+ */
+int lk_load_kv_q8(void* key_out, void* value_out, const void* k_data, const float* k_scale,
+                  const void* v_data, const float* v_scale, const int32_t* block_tables,
+                  int64_t block_table_stride, const int32_t* context_lens,
+                  const int32_t* cu_rows, int32_t num_seqs, int64_t num_rows, int32_t H_kv,
+                  int32_t D, int64_t num_blocks, int32_t block_size,
+                  int32_t max_blocks_per_seq, int32_t dtype, int32_t kv_format,
+                  int32_t* status, void* stream);
 
 /*
  * Paged decode attention. Replaces Attention._decode_fast,
@@ -245,6 +292,89 @@ int lk_paged_prefill_ws(void* out, const void* q, int64_t q_token_stride,
                         int32_t H, int32_t H_kv, int32_t D, int32_t block_size,
                         float scale, int32_t dtype, void* workspace, size_t workspace_bytes,
                         int32_t* status, void* stream);
+
+/*
+ * Attention of a tree of drafted tokens over the paged cache (speculative
+ * decoding). No counterpart in the reference. Sequence b has
+ * n = cu_seqlens_q[b+1] - cu_seqlens_q[b] query tokens (rows cu_seqlens_q[b]..
+ * of q / out, [num_tokens, H, D], head stride D), n <= max_q_len, whose keys and
+ * values are already stored as the last n of its context_lens[b] tokens. Token
+ * i sees every key before those n, and the d-th of them where bit d of its mask
+ * row is set: word d / 64 of tree_mask + row * mask_stride (int64 words, row
+ * counted over all sequences; mask_words * 64 >= max_q_len). tree_mask NULL: a
+ * chain, token i sees drafts d <= i. A token that sees no key gives NaN, as a
+ * context of 0 does in lk_paged_decode. cu_seqlens_q NULL: decode, one token
+ * per sequence (num_tokens == num_seqs, max_q_len 1, no mask).
+ * kv_format LK_KV_16BIT: caches of the query's dtype, scales ignored;
+ * LK_KV_INT8 / LK_KV_E4M3: lk_store_kv_q8's caches. dtype F16 or BF16, D 64 or
+ * 128, any block_size, any G = H / H_kv; caches 16-byte aligned. Scores,
+ * softmax and sums are fp32; weights are rounded to 16 bits before the product
+ * with V (f16 for 8-bit caches, the cache's type otherwise).
+ * Rows of out that belong to no sequence are left as they were. *status (may
+ * be NULL) receives LK_STATUS_BLOCK_OOB (a block id outside the cache: that key's
+ * row reads zeros) and LK_STATUS_CTX_OOB (a context longer than the table or
+ * shorter than n, or a cu_seqlens_q that passes num_tokens or max_q_len).
+ * workspace: lk_paged_tree_workspace_bytes(...) bytes (may be 0) of the same
+ * shape on the current device, 16-byte aligned, no zero-fill needed; it
+ * holds the partial results of contexts that are split, is written and read by
+ * this call only, and must not be shared by calls that overlap on the GPU.
+ */
+size_t lk_paged_tree_workspace_bytes(int32_t num_tokens, int32_t num_seqs, int32_t max_q_len,
+                                     int32_t H, int32_t H_kv, int32_t D, int32_t block_size,
+                                     int32_t max_blocks_per_seq);
+int lk_paged_tree_attention(void* out, int64_t out_token_stride,
+                            const void* q, int64_t q_token_stride,
+                            const void* k_cache, const float* k_scale,
+                            const void* v_cache, const float* v_scale, int64_t num_blocks,
+                            const int32_t* block_tables, int64_t block_table_stride,
+                            const int32_t* cu_seqlens_q, const int32_t* context_lens,
+                            const int64_t* tree_mask, int64_t mask_stride, int32_t mask_words,
+                            int32_t num_tokens, int32_t num_seqs, int32_t max_q_len,
+                            int32_t H, int32_t H_kv, int32_t D, int32_t block_size,
+                            int32_t max_blocks_per_seq, float scale, int32_t dtype,
+                            int32_t kv_format, void* workspace, size_t workspace_bytes,
+                            int32_t* status, void* stream);
+
+/*
+ * lk_paged_decode over an 8-bit cache: the same result as decode attention
+ * over the rows that lk_load_kv_q8 returns in fp32. Shapes and workspace as
+ * for lk_paged_tree_attention with one token per sequence.
+ */
+int lk_paged_decode_q8(void* out, int64_t out_token_stride, const void* q, int64_t q_token_stride,
+                       const void* k_data, const float* k_scale,
+                       const void* v_data, const float* v_scale, int64_t num_blocks,
+                       const int32_t* block_tables, int64_t block_table_stride,
+                       const int32_t* context_lens, int32_t B, int32_t H, int32_t H_kv,
+                       int32_t D, int32_t block_size, int32_t max_blocks_per_seq, float scale,
+                       int32_t dtype, int32_t kv_format, void* workspace,
+                       size_t workspace_bytes, int32_t* status, void* stream);
+
+/*
+ * Penalties, biases and a grammar mask on a step's logits, in one pass. For
+ * token v of row b, with c its occurrences in the row's output tokens, in fp32:
+ *   v in prompt or output: x = x > 0 ? x / repetition[b] : x * repetition[b]
+ *   x = x - (frequency[b] * c + presence[b] * (c > 0))
+ *   x = x + the sum of the biases listed for v, added in list order
+ *   bit v % 32 of word v / 32 of the row's allowed mask is 0: x = -inf
+ * and one rounding to the logits' type. The repetition step is the
+ * reference's _apply_repetition_penalty (litevllm/layers/sampler.py:190-201).
+ * Any of the operands may be NULL (off). prompt_ids / output_ids: int64
+ * [B, prompt_max] / [B, output_max] with row strides, of which the first
+ * prompt_lens[b] / output_lens[b] count (NULL: all); a negative id is padding,
+ * an id >= V is skipped and flagged LK_STATUS_TOKEN_OOB in *status (may be
+ * NULL). bias_ids int64 / bias fp32: [B, num_bias] contiguous, num_bias <= 1024, ids
+ * as above. allowed: int32 words, row stride allowed_ld. logits / out: [B, V],
+ * F32, F16 or BF16, row strides ld / out_ld; out may be logits (the same ld),
+ * and otherwise must not overlap it. B <= 65535.
+ */
+int lk_process_logits(void* out, int64_t out_ld, const void* logits, int32_t B, int32_t V,
+                      int64_t ld, const int64_t* prompt_ids, int64_t prompt_ld,
+                      const int32_t* prompt_lens, int32_t prompt_max, const int64_t* output_ids,
+                      int64_t output_ld, const int32_t* output_lens, int32_t output_max,
+                      const float* repetition, const float* presence, const float* frequency,
+                      const int64_t* bias_ids, const float* bias, int32_t num_bias,
+                      const int32_t* allowed, int64_t allowed_ld, int32_t dtype,
+                      int32_t* status, void* stream);
 
 /*
  * Vocab-wide sampler. Replaces Sampler.sample's greedy path

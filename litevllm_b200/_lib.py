@@ -16,6 +16,7 @@ LIB_PATH = Path(__file__).resolve().parent / "liblitekern.so"
 
 LK_OK = 0
 LK_DTYPE_F32, LK_DTYPE_F16, LK_DTYPE_BF16 = 0, 1, 2
+LK_KV_16BIT, LK_KV_INT8, LK_KV_E4M3 = 0, 1, 2
 LK_STATUS_SLOT_OOB = 1
 LK_STATUS_BLOCK_OOB = 2
 LK_STATUS_WAIT_TIMEOUT = 4
@@ -30,6 +31,17 @@ SIGNATURES: dict[str, tuple] = {
         c_int32,
         [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_int32, c_int32,
          c_int64, c_int64, c_int64, c_int32, c_void_p, c_void_p],
+    ),
+    "lk_store_kv_q8": (
+        c_int32,
+        [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_int32,
+         c_int32, c_int64, c_int64, c_int64, c_int32, c_int32, c_int32, c_void_p, c_void_p],
+    ),
+    "lk_load_kv_q8": (
+        c_int32,
+        [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_void_p,
+         c_void_p, c_int32, c_int64, c_int32, c_int32, c_int64, c_int32, c_int32, c_int32,
+         c_int32, c_void_p, c_void_p],
     ),
     "lk_paged_decode_num_splits": (c_int32, [c_int32, c_int32, c_int32, c_int32]),
     "lk_paged_decode_workspace_bytes": (c_size_t, [c_int32, c_int32, c_int32, c_int32, c_int32]),
@@ -68,6 +80,26 @@ SIGNATURES: dict[str, tuple] = {
         [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_int64,
          c_void_p, c_void_p, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32,
          c_float, c_int32, c_void_p, c_void_p],
+    ),
+    "lk_paged_tree_workspace_bytes": (c_size_t, [c_int32] * 8),
+    "lk_paged_tree_attention": (
+        c_int32,
+        [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_int64,
+         c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int64, c_int32, c_int32, c_int32,
+         c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, c_float, c_int32, c_int32,
+         c_void_p, c_size_t, c_void_p, c_void_p],
+    ),
+    "lk_paged_decode_q8": (
+        c_int32,
+        [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_int64,
+         c_void_p, c_int64, c_void_p, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32,
+         c_float, c_int32, c_int32, c_void_p, c_size_t, c_void_p, c_void_p],
+    ),
+    "lk_process_logits": (
+        c_int32,
+        [c_void_p, c_int64, c_void_p, c_int32, c_int32, c_int64, c_void_p, c_int64, c_void_p,
+         c_int32, c_void_p, c_int64, c_void_p, c_int32, c_void_p, c_void_p, c_void_p, c_void_p,
+         c_void_p, c_int32, c_void_p, c_int64, c_int32, c_void_p, c_void_p],
     ),
     "lk_sample_workspace_bytes": (c_size_t, [c_int32, c_int32]),
     "lk_sample": (

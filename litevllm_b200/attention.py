@@ -78,6 +78,43 @@ def set_shared_prefix_hint(block_tables: Optional[torch.Tensor], prefix_tokens: 
     _SHARED_PREFIX["tokens"] = int(prefix_tokens) if block_tables is not None else 0
 
 
+def _store(key, value, key_cache, value_cache, slot_mapping) -> None:
+    """The KV store into 16-bit caches or a QuantizedCache pair."""
+    if isinstance(key_cache, ops.QuantizedCache):
+        ops.store_kvcache_q8(key, value, key_cache, value_cache, slot_mapping)
+    else:
+        ops.store_kvcache(key, value, key_cache, value_cache, slot_mapping)
+
+
+def _prefill(query, key_cache, value_cache, cu_seqlens_q, max_q_len, scale, block_tables,
+             context_lens, out=None) -> torch.Tensor:
+    """paged_prefill over 16-bit caches or a QuantizedCache pair. The 8-bit
+    contexts are read back once into 16-bit blocks of this call's own, every
+    sequence's in order, which the prefill kernel then reads: a chunk of queries
+    uses each key many times, the copy moves it twice."""
+    if isinstance(key_cache, ops.QuantizedCache):
+        nb, bs, H_kv, D = key_cache.data.shape
+        S, blocks = block_tables.shape
+        dev = query.device
+        cu_rows = torch.arange(0, S * blocks * bs + 1, max(1, blocks * bs), dtype=torch.int32,
+                               device=dev)
+        key_cache, value_cache = (
+            x.view(S * blocks, bs, H_kv, D) for x in ops.load_kvcache_q8(
+                key_cache, value_cache, block_tables, context_lens, cu_rows, S * blocks * bs,
+                dtype=query.dtype))
+        block_tables = torch.arange(S * blocks, dtype=torch.int32, device=dev).view(S, blocks)
+    return ops.paged_prefill(query, key_cache, value_cache, cu_seqlens_q, max_q_len, scale,
+                             block_tables=block_tables, context_lens=context_lens, out=out)
+
+
+def _decode(query, key_cache, value_cache, block_tables, context_lens, scale, out=None):
+    if isinstance(key_cache, ops.QuantizedCache):
+        return ops.paged_decode_q8(query, key_cache, value_cache, block_tables, context_lens, scale,
+                                   out=out)
+    return ops.paged_decode(query, key_cache, value_cache, block_tables, context_lens, scale,
+                            out=out)
+
+
 class PagedAttention:
     """Static helpers with the reference's names (attention.py:14-65)."""
 
@@ -90,7 +127,7 @@ class PagedAttention:
         slot_mapping: torch.Tensor,
     ) -> None:
         """key_cache[slot // bs, slot % bs] = key (attention.py:18-33)."""
-        ops.store_kvcache(key, value, key_cache, value_cache, slot_mapping)
+        _store(key, value, key_cache, value_cache, slot_mapping)
 
     # north-star alias
     store_kvcache = write_to_cache
@@ -98,11 +135,15 @@ class PagedAttention:
 
 def store_kvcache(key, value, key_cache, value_cache, slot_mapping) -> None:
     """Module-level alias of the KV store (north-star name)."""
-    ops.store_kvcache(key, value, key_cache, value_cache, slot_mapping)
+    _store(key, value, key_cache, value_cache, slot_mapping)
 
 
 class Attention(nn.Module):
-    """Attention over the paged KV cache (reference: attention.py:68-151)."""
+    """Attention over the paged KV cache (reference: attention.py:68-151).
+
+    key_cache / value_cache are 16-bit (or fp32) tensors, or a pair of
+    ops.QuantizedCache: the new rows are then quantised as they are stored and
+    every path reads the 8-bit rows."""
 
     def __init__(self, num_heads, head_dim, num_kv_heads, scale=None):
         super().__init__()
@@ -143,7 +184,7 @@ class Attention(nn.Module):
                 context_lens, mixed["cu_seqlens_q"], mixed["P"], mixed["TP"], mixed["max_q_len"])
 
         if slot_mapping is not None and key_cache is not None:
-            ops.store_kvcache(key, value, key_cache, value_cache, slot_mapping)
+            _store(key, value, key_cache, value_cache, slot_mapping)
 
         if is_prefill:
             if block_table is None:
@@ -163,7 +204,7 @@ class Attention(nn.Module):
                 # back from cu_seqlens_q would wait for the device; query tiles
                 # past a chunk's end take no work
                 max_q_len = query.shape[0]
-            return ops.paged_prefill(
+            return _prefill(
                 query, key_cache, value_cache, cu_seqlens_q, max_q_len, self.scale,
                 block_tables=block_table, context_lens=context_lens,
             )
@@ -171,6 +212,7 @@ class Attention(nn.Module):
         pref = _SHARED_PREFIX["tokens"]
         if (
             pref >= SHARED_PREFIX_MIN_TOKENS
+            and not isinstance(key_cache, ops.QuantizedCache)
             and block_table is _SHARED_PREFIX["table"]
             and query.shape[0] >= SHARED_PREFIX_MIN_ROWS
             and ops.tuned_attention_shape(query.dtype, self.head_dim, key_cache.shape[1],
@@ -180,9 +222,31 @@ class Attention(nn.Module):
             return ops.paged_decode_shared_prefix(
                 query, key_cache, value_cache, block_table, context_lens, self.scale, pref
             )
-        return ops.paged_decode(
-            query, key_cache, value_cache, block_table, context_lens, self.scale
-        )
+        return _decode(query, key_cache, value_cache, block_table, context_lens, self.scale)
+
+    def forward_tree(
+        self,
+        query: torch.Tensor,
+        key: torch.Tensor,
+        value: torch.Tensor,
+        key_cache,
+        value_cache,
+        block_table: torch.Tensor,
+        slot_mapping: Optional[torch.Tensor],
+        context_lens: torch.Tensor,
+        cu_seqlens_q: torch.Tensor,
+        max_q_len: int,
+        tree_mask: Optional[torch.Tensor] = None,
+    ) -> torch.Tensor:
+        """One step that checks drafted tokens: rows cu_seqlens_q[b].. are
+        sequence b's drafted tokens, the last of its context_lens[b] tokens. Their
+        K/V are stored, then each attends the context before them and the drafted
+        tokens its row of tree_mask names (ops.tree_mask_from_parents; None: a
+        chain). No counterpart in the reference."""
+        if slot_mapping is not None and key_cache is not None:
+            _store(key, value, key_cache, value_cache, slot_mapping)
+        return ops.paged_tree_attention(query, key_cache, value_cache, block_table, context_lens,
+                                        cu_seqlens_q, max_q_len, self.scale, tree_mask=tree_mask)
 
     def forward_mixed(
         self,
@@ -209,21 +273,19 @@ class Attention(nn.Module):
         before returning.
         """
         if slot_mapping is not None:
-            ops.store_kvcache(key, value, key_cache, value_cache, slot_mapping)
+            _store(key, value, key_cache, value_cache, slot_mapping)
         out = torch.empty_like(query)
         P, TP = num_prefill_seqs, num_prefill_tokens
 
         def prefill():
-            ops.paged_prefill(
+            _prefill(
                 query[:TP], key_cache, value_cache, cu_seqlens_q[: P + 1], max_q_len, self.scale,
                 block_tables=block_table[:P], context_lens=context_lens[:P], out=out[:TP],
             )
 
         def decode():
-            ops.paged_decode(
-                query[TP:], key_cache, value_cache, block_table[P:], context_lens[P:], self.scale,
-                out=out[TP:],
-            )
+            _decode(query[TP:], key_cache, value_cache, block_table[P:], context_lens[P:],
+                    self.scale, out=out[TP:])
 
         has_p, has_d = P > 0, query.shape[0] > TP
         if has_p and has_d and MIXED_OVERLAP:

@@ -126,6 +126,16 @@ LK_DEVINL void cp_async16(void* smem_dst, const void* gsrc, bool valid) {
                "l"(gsrc), "r"(valid ? 16 : 0)
                : "memory");
 }
+// 4-byte form (through L1: cp.async.cg takes 16 bytes only).
+LK_DEVINL void cp_async4(void* smem_dst, const void* gsrc, bool valid) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_u32(smem_dst)),
+               "l"(gsrc), "r"(valid ? 4 : 0)
+               : "memory");
+}
+LK_DEVINL void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> LK_DEVINL void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
 LK_DEVINL void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
 // ------------------------------------------------------------------- TMA ---

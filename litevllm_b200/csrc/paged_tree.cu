@@ -1,0 +1,277 @@
+// Entry points of drafted-tree attention and of decode over an 8-bit cache:
+// argument checks, the split plan and the kernel that joins the splits. The
+// attention kernel itself is in paged_tree.cuh.
+#include <algorithm>
+
+#include "lk_common.cuh"
+#include "paged_tree.h"
+
+namespace lk {
+namespace {
+
+struct JoinParams {
+  void* out;
+  int64_t out_stride;
+  const float4* part_ml;  // [T * H][nsplit]: m, l, M
+  const float* part_o;    // [T * H][nsplit][D]
+  const int32_t* cu_seqlens_q;
+  const int32_t* context_lens;
+  int B, H, nsplit, chunk, max_keys, max_q;
+};
+
+template <typename T> LK_DEVINL T join_round(float x);
+template <> LK_DEVINL __nv_bfloat16 join_round<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+template <> LK_DEVINL __half join_round<__half>(float x) { return __float2half_rn(x); }
+
+// out = sum_s O_s 2^(M_s - M) / sum_s l_s 2^(m_s - m) * 2^(M - m), in split
+// order whatever order the splits ended in. One CTA per query row; W warps
+// share its splits (few splits: one warp, many rows; many: four).
+template <typename T, int D, int W>
+__global__ void __launch_bounds__(W * 32) tree_join_kernel(const JoinParams p) {
+  pdl_wait();
+  const int64_t row = blockIdx.x;
+  const int t = static_cast<int>(row / p.H), h = static_cast<int>(row % p.H);
+  int b = t;
+  if (p.cu_seqlens_q) {
+    if (t < p.cu_seqlens_q[0] || t >= p.cu_seqlens_q[p.B]) return;
+    int lo = 0, hi = p.B;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (p.cu_seqlens_q[mid] <= t) lo = mid;
+      else hi = mid;
+    }
+    b = lo;
+    if (t - p.cu_seqlens_q[b] >= p.max_q) return;  // not computed
+  }
+  const int ctx = max(min(p.context_lens[b], p.max_keys), 0);
+  const int ns = (ctx + p.chunk - 1) / p.chunk;
+  if (ns <= 1) return;  // written by its only split
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const float4* ml = p.part_ml + row * p.nsplit;
+  float a = -3.402823466e38f, A = a;
+  for (int s = lane; s < ns; s += 32) {
+    const float4 w = ml[s];
+    a = fmaxf(a, w.x);
+    A = fmaxf(A, w.z);
+  }
+  a = warp_max(a);
+  A = warp_max(A);
+  constexpr int V = D / 32;
+  float acc[V], L = 0.f;
+#pragma unroll
+  for (int i = 0; i < V; ++i) acc[i] = 0.f;
+#pragma unroll 4
+  for (int s = warp; s < ns; s += W) {
+    const float4 w = ml[s];
+    const float f = ex2_mufu(w.z - A);
+    L += w.y * ex2_mufu(w.x - a);
+    const float* po = p.part_o + (row * p.nsplit + s) * D + lane * V;
+#pragma unroll
+    for (int i = 0; i < V; i += 2) {
+      const float2 x = *reinterpret_cast<const float2*>(po + i);
+      acc[i] += x.x * f;
+      acc[i + 1] += x.y * f;
+    }
+  }
+  if constexpr (W > 1) {
+    __shared__ float sm[W][D + 1];
+#pragma unroll
+    for (int i = 0; i < V; ++i) sm[warp][lane * V + i] = acc[i];
+    if (lane == 0) sm[warp][D] = L;
+    __syncthreads();
+    if (warp != 0) return;
+    L = 0.f;
+#pragma unroll
+    for (int i = 0; i < V; ++i) acc[i] = 0.f;
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      L += sm[w][D];
+#pragma unroll
+      for (int i = 0; i < V; ++i) acc[i] += sm[w][lane * V + i];
+    }
+  }
+  const float fin = exp2f(A - a) / L;
+  T* dst = static_cast<T*>(p.out) + t * p.out_stride + h * D + lane * V;
+#pragma unroll
+  for (int i = 0; i < V; ++i) dst[i] = join_round<T>(acc[i] * fin);
+}
+
+struct Plan {
+  int NT, chunk, nsplit;
+  int64_t grid;
+};
+
+// Query rows per CTA: the smallest of 8, 16, 32 that holds a KV head's rows
+// (32 re-reads the keys from L2 for every 32 rows). Splits: enough for two
+// waves of CTAs when every context is as long as the table, pieces of at
+// least 256 keys (a warp's ramp of ~2 us costs as much as ~64 keys a warp) and
+// at most 2048, so that a batch of mixed lengths ends evenly; longer pieces
+// again where a wide table would make more than 65536 CTAs, most of them empty.
+Plan plan_of(int B, int max_q, int H, int H_kv, int bs, int max_blocks) {
+  Plan r;
+  const int rows = max_q * (H / H_kv);
+  r.NT = rows <= 8 ? 1 : rows <= 16 ? 2 : 4;
+  const int64_t units =
+      static_cast<int64_t>(B) * H_kv * ((rows + 8 * r.NT - 1) / (8 * r.NT));
+  const int64_t keys = std::max<int64_t>(1, static_cast<int64_t>(max_blocks) * bs);
+  const int64_t slots = static_cast<int64_t>(num_sms()) * (r.NT == 1 ? 3 : 2);
+  const int64_t want = std::max<int64_t>(1, (2 * slots + units - 1) / units);
+  auto round_up = [](int64_t x, int64_t m) { return (x + m - 1) / m * m; };
+  int64_t chunk = round_up((keys + want - 1) / want, 128);
+  chunk = std::min<int64_t>(std::max<int64_t>(chunk, 256), 2048);
+  const int64_t most = std::max<int64_t>(1, 65536 / units);
+  chunk = std::max(chunk, round_up((keys + most - 1) / most, 128));
+  r.chunk = static_cast<int>(std::min<int64_t>(chunk, 1 << 30));
+  r.nsplit = static_cast<int>((keys + r.chunk - 1) / r.chunk);
+  r.grid = units * r.nsplit;
+  return r;
+}
+
+size_t plan_bytes(const Plan& r, int64_t T, int H, int D) {
+  return r.nsplit == 1 ? 0 : static_cast<size_t>(T) * H * r.nsplit * (D + 4) * 4;
+}
+
+template <typename T, int D>
+cudaError_t join(const JoinParams& j, unsigned rows, cudaStream_t s) {
+  if (j.nsplit <= 8)
+    return launch_after_previous(tree_join_kernel<T, D, 1>, dim3(rows), dim3(32), 0, s, j);
+  return launch_after_previous(tree_join_kernel<T, D, 4>, dim3(rows), dim3(128), 0, s, j);
+}
+
+int run(TreeParams& p, int T, int H, int D, float scale, int dtype, int fmt, void* workspace,
+        size_t workspace_bytes, cudaStream_t s) {
+  const Plan r = plan_of(p.B, p.max_q, H, p.H_kv, p.bs, p.max_blocks);
+  if (r.grid > 0x7fffffffLL || static_cast<int64_t>(T) * H > 0x7fffffffLL) return LK_ERR_INVALID_ARG;
+  const size_t need = plan_bytes(r, T, H, D);
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need ||
+                   (reinterpret_cast<uintptr_t>(workspace) & 15u) != 0))
+    return LK_ERR_WORKSPACE;
+  p.scale_log2 = scale * 1.4426950408889634f;
+  p.chunk = r.chunk;
+  p.nsplit = r.nsplit;
+  p.part_ml = static_cast<float4*>(workspace);
+  p.part_o = r.nsplit == 1 ? nullptr
+                           : reinterpret_cast<float*>(p.part_ml + static_cast<int64_t>(T) * H * r.nsplit);
+  const unsigned grid = static_cast<unsigned>(r.grid);
+  int rc = fmt == LK_KV_16BIT  ? tree_launch_16(p, dtype, D, r.NT, grid, s)
+           : fmt == LK_KV_INT8 ? tree_launch_i8(p, dtype, D, r.NT, grid, s)
+                               : tree_launch_e4m3(p, dtype, D, r.NT, grid, s);
+  if (rc != LK_OK || r.nsplit == 1) return rc;
+  JoinParams j;
+  j.out = p.out;
+  j.out_stride = p.out_stride;
+  j.part_ml = p.part_ml;
+  j.part_o = p.part_o;
+  j.cu_seqlens_q = p.cu_seqlens_q;
+  j.context_lens = p.context_lens;
+  j.B = p.B;
+  j.H = H;
+  j.nsplit = r.nsplit;
+  j.chunk = r.chunk;
+  j.max_keys = p.max_blocks * p.bs;
+  j.max_q = p.max_q;
+  const unsigned rows = static_cast<unsigned>(T) * H;
+  cudaError_t e;
+  if (dtype == LK_DTYPE_BF16)
+    e = D == 128 ? join<__nv_bfloat16, 128>(j, rows, s) : join<__nv_bfloat16, 64>(j, rows, s);
+  else
+    e = D == 128 ? join<__half, 128>(j, rows, s) : join<__half, 64>(j, rows, s);
+  return e == cudaSuccess ? check_launch() : LK_ERR_CUDA;
+}
+
+bool shape_ok(int H, int H_kv, int D, int bs, int max_blocks, int64_t num_blocks, int dtype,
+              int fmt, int* rc) {
+  *rc = LK_OK;
+  if (H <= 0 || H_kv <= 0 || H % H_kv != 0 || bs <= 0 || max_blocks <= 0 || num_blocks < 0) {
+    *rc = LK_ERR_INVALID_ARG;
+  } else if ((D != 64 && D != 128) || (dtype != LK_DTYPE_F16 && dtype != LK_DTYPE_BF16) ||
+             (fmt != LK_KV_16BIT && fmt != LK_KV_INT8 && fmt != LK_KV_E4M3) ||
+             num_blocks > 0x7fffffffLL / bs || max_blocks > 0x7fff0000 / bs) {
+    *rc = LK_ERR_UNSUPPORTED;
+  }
+  return *rc == LK_OK;
+}
+
+bool aligned(const void* a) { return (reinterpret_cast<uintptr_t>(a) & 15u) == 0; }
+
+}  // namespace
+}  // namespace lk
+
+extern "C" size_t lk_paged_tree_workspace_bytes(int32_t num_tokens, int32_t num_seqs,
+                                                int32_t max_q_len, int32_t H, int32_t H_kv,
+                                                int32_t D, int32_t block_size,
+                                                int32_t max_blocks_per_seq) {
+  if (num_tokens <= 0 || num_seqs <= 0 || max_q_len <= 0 || H <= 0 || H_kv <= 0 ||
+      H % H_kv != 0 || D <= 0 || block_size <= 0 || max_blocks_per_seq <= 0)
+    return 0;
+  return lk::plan_bytes(
+      lk::plan_of(num_seqs, max_q_len, H, H_kv, block_size, max_blocks_per_seq), num_tokens, H, D);
+}
+
+extern "C" int lk_paged_tree_attention(
+    void* out, int64_t out_token_stride, const void* q, int64_t q_token_stride,
+    const void* k_cache, const float* k_scale, const void* v_cache, const float* v_scale,
+    int64_t num_blocks, const int32_t* block_tables, int64_t block_table_stride,
+    const int32_t* cu_seqlens_q, const int32_t* context_lens, const int64_t* tree_mask,
+    int64_t mask_stride, int32_t mask_words, int32_t num_tokens, int32_t num_seqs,
+    int32_t max_q_len, int32_t H, int32_t H_kv, int32_t D, int32_t block_size,
+    int32_t max_blocks_per_seq, float scale, int32_t dtype, int32_t kv_format, void* workspace,
+    size_t workspace_bytes, int32_t* status, void* stream) {
+  int rc;
+  if (num_tokens < 0 || num_seqs < 0 || max_q_len < 0) return LK_ERR_INVALID_ARG;
+  if (!lk::shape_ok(H, H_kv, D, block_size, max_blocks_per_seq, num_blocks, dtype, kv_format, &rc))
+    return rc;
+  if (num_tokens == 0 || num_seqs == 0 || max_q_len == 0) return LK_OK;
+  const bool q8 = kv_format != LK_KV_16BIT;
+  if (!out || !q || !k_cache || !v_cache || !block_tables || !context_lens ||
+      (q8 && (!k_scale || !v_scale)) || (!cu_seqlens_q && (max_q_len != 1 || tree_mask)) ||
+      (!cu_seqlens_q && num_tokens != num_seqs) ||
+      (tree_mask && (mask_words <= 0 || static_cast<int64_t>(mask_words) * 64 < max_q_len)) ||
+      static_cast<int64_t>(max_q_len) * (H / H_kv) > 0x7fffffffLL / 2)
+    return LK_ERR_INVALID_ARG;
+  if (!lk::aligned(k_cache) || !lk::aligned(v_cache)) return LK_ERR_ALIGNMENT;
+  lk::TreeParams p = {};
+  p.out = out;
+  p.out_stride = out_token_stride;
+  p.q = q;
+  p.q_stride = q_token_stride;
+  p.k = k_cache;
+  p.v = v_cache;
+  p.k_scale = k_scale;
+  p.v_scale = v_scale;
+  p.block_tables = block_tables;
+  p.bt_stride = block_table_stride;
+  p.context_lens = context_lens;
+  p.cu_seqlens_q = cu_seqlens_q;
+  p.mask = tree_mask;
+  p.mask_stride = mask_stride;
+  p.mask_words = mask_words;
+  p.status = status;
+  p.T = num_tokens;
+  p.B = num_seqs;
+  p.H_kv = H_kv;
+  p.G = H / H_kv;
+  p.bs = block_size;
+  p.max_blocks = max_blocks_per_seq;
+  p.num_blocks = num_blocks;
+  p.max_q = max_q_len;
+  return lk::run(p, num_tokens, H, D, scale, dtype, kv_format, workspace, workspace_bytes,
+                 static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int lk_paged_decode_q8(void* out, int64_t out_token_stride, const void* q,
+                                  int64_t q_token_stride, const void* k_data,
+                                  const float* k_scale, const void* v_data, const float* v_scale,
+                                  int64_t num_blocks, const int32_t* block_tables,
+                                  int64_t block_table_stride, const int32_t* context_lens,
+                                  int32_t B, int32_t H, int32_t H_kv, int32_t D,
+                                  int32_t block_size, int32_t max_blocks_per_seq, float scale,
+                                  int32_t dtype, int32_t kv_format, void* workspace,
+                                  size_t workspace_bytes, int32_t* status, void* stream) {
+  if (kv_format == LK_KV_16BIT) return LK_ERR_UNSUPPORTED;  // lk_paged_decode reads those
+  return lk_paged_tree_attention(out, out_token_stride, q, q_token_stride, k_data, k_scale,
+                                 v_data, v_scale, num_blocks, block_tables, block_table_stride,
+                                 nullptr, context_lens, nullptr, 0, 0, B, B, 1, H, H_kv, D,
+                                 block_size, max_blocks_per_seq, scale, dtype, kv_format,
+                                 workspace, workspace_bytes, status, stream);
+}

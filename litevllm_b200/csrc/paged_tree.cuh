@@ -1,0 +1,645 @@
+// Attention of a few query tokens per sequence over the paged cache: a tree of
+// drafted tokens (16-bit or 8-bit cache) and single-token decode over an 8-bit
+// cache.
+//
+// Sequence b has n query tokens at the end of its context of ctx tokens, all
+// already stored; token i sees every key j < ctx - n and key ctx - n + j where
+// bit j of its mask row is set (no mask: j <= i). For its query heads,
+//   out = sum_j p_j s_v[j] v[j] / sum_j p_j,  p_j = exp(scale s_k[j] q.k[j]),
+// s = 1 for 16-bit caches. GQA: the n * G query rows of a KV head share its keys.
+//
+// The keys are read once for up to 32 query rows and 4 H D operations a key, so
+// HBM bounds it while n * G is small. Layout:
+//  * CTA = (KV head, 8 NT query rows, split of the context, sequence), four
+//    warps. Each warp streams its own stages of kTok keys (warp w takes stages
+//    w, w + 4, ...) with 16-byte cp.async through a private ring: no barrier
+//    between warps until the end, any block size, rows past the split are
+//    zero-filled and never read.
+//  * S^T = K Q^T (16 keys x 8 query rows) and O^T += V^T P^T on mma.sync
+//    m16n8k16 with fp32 accumulators. 8-bit rows become f16 in registers, exactly:
+//    a 16-byte piece of a K row is one k-step whose slots are permuted the same
+//    way in Q, and ldmatrix.trans on byte pairs gives V^T tiles whose rows are
+//    the even and the odd d of the pair. The scales stay out of the products:
+//    s_k multiplies the score, log2 s_v joins the exponent of the weight, so
+//    the weights keep f16's 11 bits whatever the rows' sizes. Q is scaled by a
+//    power of two per row into f16's range.
+//  * Online softmax in base 2, with the running maximum raised only when some
+//    score exceeds it by 2^8 (weights up to 256 are as exact as weights up to
+//    1, and the vote costs one instruction where the maximum costs six shuffles).
+//    8-bit caches hold two: m for the sum of p, M for the weights p s_v, which
+//    are rounded to f16 relative to their own maximum. Sums stay in fp32.
+//  * Splits write (m, l, M, O) and a second small kernel joins them; a sequence
+//    that fits one split is written directly.
+#pragma once
+
+#include <type_traits>
+
+#include "lk_q8.cuh"
+#include "paged_tree.h"
+
+namespace lk {
+namespace tree {
+
+constexpr int kWarps = 4;
+constexpr float kRaise = 8.f;  // log2 of the largest weight
+
+template <int FMT, typename T> struct MmaType { using type = __half; };
+template <typename T> struct MmaType<LK_KV_16BIT, T> { using type = T; };
+
+template <int FMT, int D> struct Shape {
+  static constexpr int kEsz = FMT == LK_KV_16BIT ? 2 : 1;
+  static constexpr int kRow = D * kEsz;       // bytes of a key row
+  static constexpr int kCpr = kRow / 16;      // 16-byte pieces of a row
+  static constexpr int kTok = kEsz == 1 ? 32 : 16;  // keys per stage: 8 KB of K and V at D = 128
+  static constexpr int kMt = kTok / 16;
+  static constexpr int kNst = 3;
+  static constexpr int kTile = kTok * kRow;
+  static constexpr int kScales = kEsz == 1 ? 2 * kTok * 4 : 0;
+  static constexpr int kStage = 2 * kTile + kScales;
+  static constexpr int kRing = kWarps * kNst * kStage;
+};
+
+// Byte offset of piece `c` of row `r`: XOR-swizzled so that the eight rows of an
+// ldmatrix at one piece fall into different 16-byte bank groups.
+template <int CPR> LK_DEVINL uint32_t piece(uint32_t r, uint32_t c) {
+  const uint32_t f = CPR >= 8 ? (r & 7u) : ((r >> 1) & 3u);
+  return (r * CPR + (c ^ f)) << 4;
+}
+
+// Whether a 16-bit value, or either half of a pair, is an infinity or a NaN.
+template <typename T> LK_DEVINL bool has_special(uint32_t w) {
+  constexpr uint32_t e = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
+  return (w & e) == e || (w & (e << 16)) == (e << 16);
+}
+template <typename T> LK_DEVINL float from_16(uint32_t b) {
+  const uint16_t h = static_cast<uint16_t>(b);
+  return Elem<T>::to_f(*reinterpret_cast<const T*>(&h));
+}
+
+template <typename T> LK_DEVINL T round_to(float x);
+template <> LK_DEVINL __nv_bfloat16 round_to<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+template <> LK_DEVINL __half round_to<__half>(float x) { return __float2half_rn(x); }
+
+template <int FMT, typename T, int D, int NT> struct Smem {
+  static constexpr int kCols = 8 * NT;
+  static constexpr int kQStride = D * 2 + 16;  // bytes; rows shift by 16 bytes: no bank conflicts
+  static constexpr int kMerge = kWarps * kCols * (D + 4) * 4 + kWarps * kCols * 16;
+  static constexpr int kMain = Shape<FMT, D>::kRing > kMerge ? Shape<FMT, D>::kRing : kMerge;
+  static constexpr int kBytes = kMain + kCols * kQStride + kCols * 12;
+};
+
+template <int FMT, typename T, int D, int NT>
+__global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 2)
+paged_tree_kernel(const TreeParams p) {
+  using S = Shape<FMT, D>;
+  using SM = Smem<FMT, T, D, NT>;
+  using MT = typename MmaType<FMT, T>::type;
+  constexpr bool Q8B = FMT != LK_KV_16BIT;
+  constexpr int COLS = 8 * NT;
+  constexpr int KS = D / 16;
+  extern __shared__ __align__(16) uint8_t smem[];
+  uint8_t* q_smem = smem + SM::kMain;
+  float* col_scale = reinterpret_cast<float*>(q_smem + COLS * SM::kQStride);
+  int* col_token = reinterpret_cast<int*>(col_scale + COLS);  // query token of a column, -1: none
+  int* col_head = col_token + COLS;
+
+  // Waits for the kernel ahead (the store of this step's rows).
+  pdl_wait();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int g = lane >> 2, c = lane & 3;
+
+  const int col_groups = (p.max_q * p.G + COLS - 1) / COLS;
+  unsigned u = blockIdx.x;
+  const int cg = u % col_groups;
+  u /= col_groups;
+  const int kvh = u % p.H_kv;
+  u /= p.H_kv;
+  const int b = u % p.B;
+  const int sp = u / p.B;
+
+  int row0 = b, n = 1;
+  if (p.cu_seqlens_q) {
+    row0 = p.cu_seqlens_q[b];
+    n = p.cu_seqlens_q[b + 1] - row0;
+    if (n > p.max_q || row0 < 0 || row0 + n > p.T) {  // a bad cu_seqlens_q: nothing outside q
+      if (threadIdx.x == 0 && p.status) atomicOr(p.status, LK_STATUS_CTX_OOB);
+      n = row0 < 0 ? 0 : min(min(n, p.max_q), p.T - row0);
+    }
+  }
+  const int rows = n * p.G;  // query rows of this KV head
+  if (cg * COLS >= rows) return;
+  int ctx = p.context_lens[b];
+  if (ctx > p.max_blocks * p.bs || ctx < (p.cu_seqlens_q ? n : 0)) {
+    if (threadIdx.x == 0 && p.status) atomicOr(p.status, LK_STATUS_CTX_OOB);
+    ctx = max(min(ctx, p.max_blocks * p.bs), 0);
+  }
+  const int key0 = sp * p.chunk;
+  if (key0 >= ctx && sp > 0) return;
+  const int key1 = min(ctx, key0 + p.chunk);
+  // keys below `open` are seen by every row
+  const int open = p.cu_seqlens_q ? max(ctx - n, 0) : ctx;
+
+  // ------------------------------------------------------------ the ring ---
+  const int64_t width = static_cast<int64_t>(p.H_kv) * S::kRow;  // bytes of a slot
+  const uint8_t* kbase = static_cast<const uint8_t*>(p.k) + kvh * S::kRow;
+  const uint8_t* vbase = static_cast<const uint8_t*>(p.v) + kvh * S::kRow;
+  const int32_t* bt = p.block_tables + static_cast<int64_t>(b) * p.bt_stride;
+  uint8_t* ring = smem + warp * (S::kNst * S::kStage);
+  const int nstage = (key1 - key0 + S::kTok - 1) / S::kTok;
+  const int mine = nstage > warp ? (nstage - warp + kWarps - 1) / kWarps : 0;
+  auto first_key = [&](int i) { return key0 + (warp + i * kWarps) * S::kTok; };
+  // Block of the lane's key of stage i: looked up one stage before its copies.
+  auto block_of = [&](int i) {
+    const int key = first_key(i) + lane;
+    if (i >= mine || lane >= S::kTok || key >= key1) return -1;
+    const int blk = __ldg(bt + key / p.bs);
+    if (blk < 0 || blk >= p.num_blocks) {
+      if (p.status) atomicOr(p.status, LK_STATUS_BLOCK_OOB);
+      return -1;
+    }
+    return blk;
+  };
+  auto load_stage = [&](int i, int blk) {
+    uint8_t* st = ring + (i % S::kNst) * S::kStage;
+    const int off = (first_key(i) + lane) % p.bs;
+    const int slot = blk < 0 ? -1 : blk * p.bs + off;
+    constexpr int RPI = 32 / S::kCpr;  // rows per copy instruction
+    const int pc = lane % S::kCpr;
+#pragma unroll
+    for (int j = 0; j < S::kTok / RPI; ++j) {
+      const int r = j * RPI + lane / S::kCpr;
+      const int sl = __shfl_sync(0xffffffffu, slot, r);
+      const int64_t at = sl < 0 ? 0 : sl * width + pc * 16;
+      const uint32_t to = piece<S::kCpr>(r, pc);
+      cp_async16(st + to, kbase + at, sl >= 0);
+      cp_async16(st + S::kTile + to, vbase + at, sl >= 0);
+    }
+    if constexpr (Q8B) {
+      float* sc = reinterpret_cast<float*>(st + 2 * S::kTile);
+      const int64_t at = slot < 0 ? 0 : (static_cast<int64_t>(blk) * p.H_kv + kvh) * p.bs + off;
+      cp_async4(sc + lane, p.k_scale + at, slot >= 0);
+      cp_async4(sc + S::kTok + lane, p.v_scale + at, slot >= 0);
+    }
+  };
+  int next = block_of(0);
+#pragma unroll
+  for (int i = 0; i < S::kNst - 1; ++i) {
+    const int blk = next;
+    next = block_of(i + 1);
+    if (i < mine) load_stage(i, blk);
+    cp_async_commit();
+  }
+
+  // ------------------------------------------------------ queries to smem ---
+  for (int j = warp; j < COLS; j += kWarps) {
+    const int r = cg * COLS + j;
+    const int token = r < rows ? r / p.G : -1;
+    const int head = kvh * p.G + r % p.G;
+    const T* src = static_cast<const T*>(p.q) +
+                   static_cast<int64_t>(row0 + max(token, 0)) * p.q_stride +
+                   static_cast<int64_t>(head) * D;
+    float x[D / 32], top = 0.f;
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) {
+      x[i] = token >= 0 ? Elem<T>::to_f(src[lane + 32 * i]) : 0.f;
+      top = fmaxf(top, fabsf(x[i]));
+    }
+    float up = 1.f, down = 1.f;
+    if constexpr (Q8B) {
+      top = warp_max(top);
+      // 2^k that brings the row's largest value into [2^14, 2^15); at most 2^126
+      const int e = __float_as_int(top) >> 23;
+      if (e > 0 && e < 255) {
+        const int f = min(268 - e, 253);
+        up = __int_as_float(f << 23);
+        down = __int_as_float((254 - f) << 23);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) {
+      const int d = lane + 32 * i;
+      int at = d;
+      if constexpr (Q8B) {  // bytes 4c..4c+3 of a piece feed slots 2c, 2c+1, 2c+8, 2c+9
+        const int e = d & 3, cc = (d & 15) >> 2;
+        at = (d & ~15) + (e < 2 ? 2 * cc + e : 8 + 2 * cc + (e - 2));
+      }
+      reinterpret_cast<MT*>(q_smem + j * SM::kQStride)[at] = round_to<MT>(x[i] * up);
+    }
+    if (lane == 0) {
+      col_scale[j] = p.scale_log2 * down;
+      col_token[j] = token;
+      col_head[j] = head;
+    }
+  }
+  __syncthreads();
+
+  // Q^T operand: registers while they fit, else read from smem per stage
+  constexpr bool QREG = NT <= 2;
+  uint32_t qf[QREG ? NT : 1][QREG ? KS : 1][2];
+  const uint32_t q_addr = smem_u32(q_smem) + (lane & 7) * SM::kQStride + (lane >> 3) * 16;
+  if constexpr (QREG) {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int i = 0; i < KS / 2; ++i)
+        ldsm_x4(q_addr + nt * 8 * SM::kQStride + i * 64, qf[nt][2 * i][0], qf[nt][2 * i][1],
+                qf[nt][2 * i + 1][0], qf[nt][2 * i + 1][1]);
+  }
+  float cs[NT][2];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    cs[nt][0] = col_scale[nt * 8 + 2 * c];
+    cs[nt][1] = col_scale[nt * 8 + 2 * c + 1];
+  }
+
+  float o[KS][NT][4];
+#pragma unroll
+  for (int i = 0; i < KS; ++i)
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) o[i][nt][0] = o[i][nt][1] = o[i][nt][2] = o[i][nt][3] = 0.f;
+  // Start of the running maxima: finite, so that a masked score (-inf) less it
+  // is -inf and never NaN.
+  float m[NT][2], l[NT][2], M[NT][2];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      m[nt][h] = M[nt][h] = -3.402823466e38f;
+      l[nt][h] = 0.f;
+    }
+
+  // Which of the keys t0 .. t0 + 31 column j sees, one bit each: all below
+  // `open`, drafted key d = key - open by the mask, none from key1 on.
+  auto window = [&](int j, int t0) {
+    const int s = t0 - open;  // > -32 where drafts matter
+    uint32_t bits = 0xffffffffu;
+    if (s > -32) {
+      const int token = col_token[j];
+      const int lo = max(s, 0);
+      uint32_t w = 0u;
+      if (token >= 0) {
+        if (p.mask == nullptr) {
+          const int k = token + 1 - lo;  // drafts lo .. token
+          w = k <= 0 ? 0u : k >= 32 ? 0xffffffffu : (1u << k) - 1u;
+        } else {
+          const int64_t* row = p.mask + static_cast<int64_t>(row0 + token) * p.mask_stride;
+          const int at = lo >> 6, sh = lo & 63;
+          const uint64_t a = at < p.mask_words ? static_cast<uint64_t>(__ldg(row + at)) : 0ull;
+          const uint64_t n = sh > 32 && at + 1 < p.mask_words
+                                 ? static_cast<uint64_t>(__ldg(row + at + 1)) << (64 - sh)
+                                 : 0ull;
+          w = static_cast<uint32_t>((a >> sh) | n);
+        }
+      }
+      bits = s >= 0 ? w : (w << -s) | ((1u << -s) - 1u);
+    }
+    const int left = key1 - t0;
+    return left >= 32 ? bits : bits & ((1u << left) - 1u);
+  };
+
+  const int lj = lane >> 3;
+  for (int i = 0; i < mine; ++i) {
+    {
+      const int ahead = i + S::kNst - 1;
+      const int blk = next;
+      next = block_of(ahead + 1);
+      __syncwarp();  // every lane has read the slot that is filled now
+      if (ahead < mine) load_stage(ahead, blk);
+      cp_async_commit();
+    }
+    cp_async_wait<S::kNst - 1>();
+    __syncwarp();
+    uint8_t* st = ring + (i % S::kNst) * S::kStage;
+    const uint32_t kb = smem_u32(st), vb = kb + S::kTile;
+    const float* sc_s = reinterpret_cast<const float*>(st + 2 * S::kTile);
+
+    // S^T = K Q^T
+    float x[S::kMt][NT][4];
+#pragma unroll
+    for (int mt = 0; mt < S::kMt; ++mt)
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+        x[mt][nt][0] = x[mt][nt][1] = x[mt][nt][2] = x[mt][nt][3] = 0.f;
+    const uint32_t krow = (lane & 7) + ((lj & 1) << 3);
+#pragma unroll
+    for (int kk = 0; kk < KS / 2; ++kk) {  // two k-steps
+      uint32_t qs[NT][4];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        if constexpr (QREG) {
+          qs[nt][0] = qf[nt][2 * kk][0];
+          qs[nt][1] = qf[nt][2 * kk][1];
+          qs[nt][2] = qf[nt][2 * kk + 1][0];
+          qs[nt][3] = qf[nt][2 * kk + 1][1];
+        } else {
+          ldsm_x4(q_addr + nt * 8 * SM::kQStride + kk * 64, qs[nt][0], qs[nt][1], qs[nt][2],
+                  qs[nt][3]);
+        }
+      }
+#pragma unroll
+      for (int mt = 0; mt < S::kMt; ++mt) {
+        uint32_t a0[4], a1[4];
+        if constexpr (Q8B) {
+          uint32_t r[4];
+          ldsm_x4(kb + piece<S::kCpr>(mt * 16 + krow, 2 * kk + (lj >> 1)), r[0], r[1], r[2], r[3]);
+          Q8<FMT>::halves(r[0], a0[0], a0[2]);
+          Q8<FMT>::halves(r[1], a0[1], a0[3]);
+          Q8<FMT>::halves(r[2], a1[0], a1[2]);
+          Q8<FMT>::halves(r[3], a1[1], a1[3]);
+        } else {
+          ldsm_x4(kb + piece<S::kCpr>(mt * 16 + krow, 4 * kk + (lj >> 1)), a0[0], a0[1], a0[2],
+                  a0[3]);
+          ldsm_x4(kb + piece<S::kCpr>(mt * 16 + krow, 4 * kk + 2 + (lj >> 1)), a1[0], a1[1], a1[2],
+                  a1[3]);
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          mma16816<MT>(x[mt][nt], a0, qs[nt][0], qs[nt][1]);
+          mma16816<MT>(x[mt][nt], a1, qs[nt][2], qs[nt][3]);
+        }
+      }
+    }
+
+    // scores in base 2; elements 0, 1: key g, columns 2c, 2c + 1; 2, 3: key g + 8
+    const int t0 = first_key(i);
+    float lsv[S::kMt][2];
+#pragma unroll
+    for (int mt = 0; mt < S::kMt; ++mt) {
+      float s0 = 1.f, s1 = 1.f;
+      if constexpr (Q8B) {
+        s0 = sc_s[mt * 16 + g];
+        s1 = sc_s[mt * 16 + g + 8];
+        lsv[mt][0] = __log2f(sc_s[S::kTok + mt * 16 + g]);
+        lsv[mt][1] = __log2f(sc_s[S::kTok + mt * 16 + g + 8]);
+      }
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        x[mt][nt][0] = x[mt][nt][0] * s0 * cs[nt][0];
+        x[mt][nt][1] = x[mt][nt][1] * s0 * cs[nt][1];
+        x[mt][nt][2] = x[mt][nt][2] * s1 * cs[nt][0];
+        x[mt][nt][3] = x[mt][nt][3] * s1 * cs[nt][1];
+      }
+    }
+    const bool drafts = min(t0 + S::kTok, key1) > open;
+    if (t0 + S::kTok > key1 || drafts) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint32_t bits = window(nt * 8 + 2 * c + h, t0) >> g;
+#pragma unroll
+          for (int mt = 0; mt < S::kMt; ++mt) {
+            if (!((bits >> (mt * 16)) & 1u)) x[mt][nt][h] = -INFINITY;
+            if (!((bits >> (mt * 16 + 8)) & 1u)) x[mt][nt][2 + h] = -INFINITY;
+          }
+        }
+    }
+
+    // raise the maxima when a score passes them by more than kRaise
+    bool up = false;
+#pragma unroll
+    for (int mt = 0; mt < S::kMt; ++mt)
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          up |= x[mt][nt][e] - m[nt][e & 1] > kRaise;
+          if constexpr (Q8B) up |= x[mt][nt][e] + lsv[mt][e >> 1] - M[nt][e & 1] > kRaise;
+        }
+    if (__any_sync(0xffffffffu, up)) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float a = m[nt][h], w = M[nt][h];
+#pragma unroll
+          for (int mt = 0; mt < S::kMt; ++mt) {
+            a = fmaxf(a, fmaxf(x[mt][nt][h], x[mt][nt][2 + h]));
+            if constexpr (Q8B)
+              w = fmaxf(w, fmaxf(x[mt][nt][h] + lsv[mt][0], x[mt][nt][2 + h] + lsv[mt][1]));
+          }
+#pragma unroll
+          for (int off = 4; off < 32; off <<= 1) {
+            a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, off));
+            if constexpr (Q8B) w = fmaxf(w, __shfl_xor_sync(0xffffffffu, w, off));
+          }
+          if constexpr (!Q8B) w = a;
+          l[nt][h] *= ex2_mufu(m[nt][h] - a);
+          const float al = ex2_mufu(M[nt][h] - w);
+          m[nt][h] = a;
+          M[nt][h] = w;
+#pragma unroll
+          for (int k = 0; k < KS; ++k) {
+            o[k][nt][h] *= al;
+            o[k][nt][2 + h] *= al;
+          }
+        }
+    }
+
+    // weights
+    uint32_t pb[S::kMt][NT][2];
+#pragma unroll
+    for (int mt = 0; mt < S::kMt; ++mt)
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        float w[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          w[e] = ex2_mufu(x[mt][nt][e] - m[nt][e & 1]);
+          l[nt][e & 1] += w[e];
+          if constexpr (Q8B) {
+            const float y = x[mt][nt][e];
+            // a masked weight is zero even where the row's scale is NaN
+            w[e] = y == -INFINITY ? 0.f : ex2_mufu(y + lsv[mt][e >> 1] - M[nt][e & 1]);
+          }
+        }
+        pb[mt][nt][0] = pack2<MT>(w[0], w[1]);
+        pb[mt][nt][1] = pack2<MT>(w[2], w[3]);
+      }
+
+    if constexpr (!Q8B) {
+      // A drafted token that some row does not see must not reach it through
+      // 0 * inf: rows of V with special values are taken out of the tile here
+      // and added to the rows that see them one by one (rare).
+      if (drafts) {
+        bool special = false;
+#pragma unroll
+        for (int k = 0; k < S::kTile / 512; ++k) {
+          const uint4 w = reinterpret_cast<const uint4*>(st + S::kTile)[lane + 32 * k];
+          special |= has_special<T>(w.x) | has_special<T>(w.y) | has_special<T>(w.z) |
+                     has_special<T>(w.w);
+        }
+        if (__any_sync(0xffffffffu, special)) {
+          for (int t = 0; t < S::kTok; ++t) {
+            uint16_t* vr = reinterpret_cast<uint16_t*>(st + S::kTile);
+            auto at = [&](int d) { return (piece<S::kCpr>(t, d >> 3) >> 1) + (d & 7); };
+            bool here = false;
+            for (int d = lane; d < D; d += 32) here |= has_special<T>(vr[at(d)]);
+            if (!__any_sync(0xffffffffu, here)) continue;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              // the weights of key t sit in the lanes with g = t & 7
+              const uint32_t pw =
+                  __shfl_sync(0xffffffffu, t < 8 ? pb[0][nt][0] : pb[0][nt][1], ((t & 7) << 2) | c);
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                if (!((window(nt * 8 + 2 * c + h, t0) >> t) & 1u)) continue;
+                const float w = from_16<T>(h ? pw >> 16 : pw & 0xffffu);
+#pragma unroll
+                for (int k = 0; k < KS; ++k) {
+                  o[k][nt][h] += w * from_16<T>(vr[at(k * 16 + g)]);
+                  o[k][nt][2 + h] += w * from_16<T>(vr[at(k * 16 + g + 8)]);
+                }
+              }
+            }
+            __syncwarp();
+            for (int d = lane; d < D; d += 32) vr[at(d)] = 0;
+            __syncwarp();
+          }
+        }
+      }
+    }
+
+    // O^T += V^T P^T
+#pragma unroll
+    for (int mt = 0; mt < S::kMt; ++mt) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        pb[mt][nt][0] = movmatrix_t(pb[mt][nt][0]);
+        pb[mt][nt][1] = movmatrix_t(pb[mt][nt][1]);
+      }
+      if constexpr (Q8B) {
+        const uint32_t vrow = mt * 16 + (lane & 7) + ((lj & 1) << 3);
+#pragma unroll
+        for (int k2 = 0; k2 < KS / 2; ++k2) {
+          uint32_t r[4], a[4];
+          ldsm_x4_t(vb + piece<S::kCpr>(vrow, 2 * k2 + (lj >> 1)), r[0], r[1], r[2], r[3]);
+          Q8<FMT>::halves_t(r[0], a[0], a[1]);
+          Q8<FMT>::halves_t(r[1], a[2], a[3]);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+            mma16816<MT>(o[2 * k2][nt], a, pb[mt][nt][0], pb[mt][nt][1]);
+          Q8<FMT>::halves_t(r[2], a[0], a[1]);
+          Q8<FMT>::halves_t(r[3], a[2], a[3]);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+            mma16816<MT>(o[2 * k2 + 1][nt], a, pb[mt][nt][0], pb[mt][nt][1]);
+        }
+      } else {
+        const uint32_t vrow = mt * 16 + (lane & 7) + ((lj >> 1) << 3);
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+          uint32_t a[4];
+          ldsm_x4_t(vb + piece<S::kCpr>(vrow, 2 * k + (lj & 1)), a[0], a[1], a[2], a[3]);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+            mma16816<MT>(o[k][nt], a, pb[mt][nt][0], pb[mt][nt][1]);
+        }
+      }
+    }
+  }
+  pdl_launch_dependents();
+
+  // -------------------------------------------------------- join the warps ---
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int off = 4; off < 32; off <<= 1)
+        l[nt][h] += __shfl_xor_sync(0xffffffffu, l[nt][h], off);
+  cp_async_wait<0>();
+  __syncthreads();  // the rings are idle: their space holds the partials
+  constexpr int OS = D + 4;
+  float* po = reinterpret_cast<float*>(smem);                        // [warp][col][OS]
+  float4* pm = reinterpret_cast<float4*>(po + kWarps * COLS * OS);   // [warp][col]
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int col = nt * 8 + 2 * c + h;
+      float* dst = po + (warp * COLS + col) * OS;
+#pragma unroll
+      for (int k = 0; k < KS; ++k) {
+        if constexpr (Q8B) {  // rows g and g + 8 are d = 2 g and 2 g + 1
+          *reinterpret_cast<float2*>(dst + k * 16 + 2 * g) =
+              make_float2(o[k][nt][h], o[k][nt][2 + h]);
+        } else {
+          dst[k * 16 + g] = o[k][nt][h];
+          dst[k * 16 + g + 8] = o[k][nt][2 + h];
+        }
+      }
+      if (g == 0)
+        pm[warp * COLS + col] = make_float4(m[nt][h], l[nt][h], Q8B ? M[nt][h] : m[nt][h], 0.f);
+    }
+  __syncthreads();
+  const bool whole = key0 == 0 && key1 == ctx;  // one split holds the whole context
+  for (int j = warp; j < COLS; j += kWarps) {
+    const int token = col_token[j];
+    if (token < 0) continue;
+    float4 w[kWarps];
+    float a = -3.402823466e38f, A = a;
+#pragma unroll
+    for (int i = 0; i < kWarps; ++i) {
+      w[i] = pm[i * COLS + j];
+      a = fmaxf(a, w[i].x);
+      A = fmaxf(A, w[i].z);
+    }
+    float L = 0.f, f[kWarps];
+#pragma unroll
+    for (int i = 0; i < kWarps; ++i) {
+      L += w[i].y * ex2_mufu(w[i].x - a);
+      f[i] = ex2_mufu(w[i].z - A);
+    }
+    const int64_t row = static_cast<int64_t>(row0 + token);
+    // no visible key: L = 0 and the row is 0 / 0 = NaN
+    const float fin = (Q8B ? exp2f(A - a) : 1.f) / L;
+    const int64_t part = (row * (p.H_kv * p.G) + col_head[j]) * p.nsplit + sp;
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) {
+      const int d = lane + 32 * i;
+      float acc = 0.f;
+#pragma unroll
+      for (int t = 0; t < kWarps; ++t) acc += po[(t * COLS + j) * OS + d] * f[t];
+      if (whole)
+        static_cast<T*>(p.out)[row * p.out_stride + col_head[j] * D + d] =
+            round_to<T>(acc * fin);
+      else
+        p.part_o[part * D + d] = acc;
+    }
+    if (!whole && lane == 0) p.part_ml[part] = make_float4(a, L, A, 0.f);
+  }
+}
+
+template <int FMT, typename T, int D, int NT>
+int launch(const TreeParams& p, unsigned grid, cudaStream_t s) {
+  constexpr int bytes = Smem<FMT, T, D, NT>::kBytes;
+  auto* kernel = paged_tree_kernel<FMT, T, D, NT>;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) !=
+      cudaSuccess)
+    return LK_ERR_CUDA;
+  if (launch_after_previous(kernel, dim3(grid), dim3(kWarps * 32), bytes, s, p) != cudaSuccess)
+    return LK_ERR_CUDA;
+  return check_launch();
+}
+
+template <int FMT, typename T, int D>
+int by_rows(const TreeParams& p, int NT, unsigned grid, cudaStream_t s) {
+  switch (NT) {
+    case 1: return launch<FMT, T, D, 1>(p, grid, s);
+    case 2: return launch<FMT, T, D, 2>(p, grid, s);
+    default: return launch<FMT, T, D, 4>(p, grid, s);
+  }
+}
+
+template <int FMT>
+int by_type(const TreeParams& p, int dtype, int D, int NT, unsigned grid, cudaStream_t s) {
+  if (dtype == LK_DTYPE_BF16)
+    return D == 128 ? by_rows<FMT, __nv_bfloat16, 128>(p, NT, grid, s)
+                    : by_rows<FMT, __nv_bfloat16, 64>(p, NT, grid, s);
+  return D == 128 ? by_rows<FMT, __half, 128>(p, NT, grid, s)
+                  : by_rows<FMT, __half, 64>(p, NT, grid, s);
+}
+
+}  // namespace tree
+}  // namespace lk

@@ -56,14 +56,17 @@ def fused_forward(self, hidden_states, positions, kv_cache=None, slot_mapping=No
         qw, kw, eps = self.q_norm.weight, self.k_norm.weight, float(self.q_norm.eps)
     cos, sin = _tables(self.rotary_emb)
     key_cache, value_cache = kv_cache if kv_cache is not None else (None, None)
-    store = slot_mapping is not None and key_cache is not None
+    # an 8-bit cache is written by the attention call, from the rotated k
+    quantised = isinstance(key_cache, ops.QuantizedCache)
+    store = slot_mapping is not None and key_cache is not None and not quantised
     # attention over the new tokens alone reads the rotated k itself
     contiguous = block_table is None
     ops.rope_store_kvcache(q, k, v, key_cache if store else None,
                            value_cache if store else None, slot_mapping if store else None,
-                           positions, cos, sin, qw, kw, eps, key_out=k if contiguous else None)
+                           positions, cos, sin, qw, kw, eps, key_out=k if contiguous or quantised else None)
     attn_output = self.attn(q, k, v, key_cache=key_cache, value_cache=value_cache,
-                            block_table=block_table, slot_mapping=None,
+                            block_table=block_table,
+                            slot_mapping=slot_mapping if quantised else None,
                             context_lens=context_lens, is_prefill=is_prefill)
     return self.o_proj(attn_output.reshape(T, -1))
 

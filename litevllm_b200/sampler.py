@@ -88,11 +88,16 @@ class Sampler:
         out: Optional[torch.Tensor] = None,
         top_k: Optional[torch.Tensor] = None,
         top_p: Optional[torch.Tensor] = None,
+        processing: Optional[dict] = None,
     ) -> torch.Tensor:
         """One sampler launch for a whole step: rows with temperature 0 are
         greedy, the others Gumbel-max at their own temperature; with per-row
         top_k (int32, <= 0 off) / top_p (fp32, >= 1 off) the fused filtered
-        kernel runs instead."""
+        kernel runs instead. processing: keyword arguments of
+        ops.process_logits (penalties, biases, grammar mask), applied first, to
+        a copy of the logits unless it names an `out`."""
+        if processing is not None:
+            logits = ops.process_logits(logits, **processing)
         if temperatures is not None and temperatures.dtype != torch.float32:
             temperatures = temperatures.float()
         if top_k is not None or top_p is not None:

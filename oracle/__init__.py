@@ -13,6 +13,10 @@ Nothing in the product (litevllm_b200/) imports this package.
                       Gumbel-max          restates :178, :187 (softmax(x/T) + draw) as
                                           argmax(x/T + g) for a given noise g
                       Philox4x32-10       the in-kernel noise generator, bit-exact ints
+  kv_q8.py            8-bit cache rows    } no counterpart in the reference: restated
+  tree_attention.py   drafted trees       } from the formulas in include/litekern.h
+  logits.py           logits processing   litevllm/layers/sampler.py:190-201 for the
+                                          repetition penalty, formulas for the rest
 
 Pinning: tests/golden/ holds outputs of the reference's own functions,
 imported from the reference checkout and run on CPU by

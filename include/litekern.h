@@ -321,7 +321,7 @@ int lk_paged_prefill_ws(void* out, const void* q, int64_t q_token_stride,
  */
 size_t lk_paged_tree_workspace_bytes(int32_t num_tokens, int32_t num_seqs, int32_t max_q_len,
                                      int32_t H, int32_t H_kv, int32_t D, int32_t block_size,
-                                     int32_t max_blocks_per_seq);
+                                     int32_t max_blocks_per_seq, int32_t kv_format);
 int lk_paged_tree_attention(void* out, int64_t out_token_stride,
                             const void* q, int64_t q_token_stride,
                             const void* k_cache, const float* k_scale,

@@ -81,7 +81,7 @@ SIGNATURES: dict[str, tuple] = {
          c_void_p, c_void_p, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32,
          c_float, c_int32, c_void_p, c_void_p],
     ),
-    "lk_paged_tree_workspace_bytes": (c_size_t, [c_int32] * 8),
+    "lk_paged_tree_workspace_bytes": (c_size_t, [c_int32] * 9),
     "lk_paged_tree_attention": (
         c_int32,
         [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_int64,

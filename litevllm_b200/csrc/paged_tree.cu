@@ -97,30 +97,55 @@ __global__ void __launch_bounds__(W * 32) tree_join_kernel(const JoinParams p) {
 }
 
 struct Plan {
-  int NT, chunk, nsplit;
+  int NT, cluster, chunk, nsplit;
   int64_t grid;
 };
 
-// Query rows per CTA: the smallest of 8, 16, 32 that holds a KV head's rows
-// (32 re-reads the keys from L2 for every 32 rows). Splits: enough for two
-// waves of CTAs when every context is as long as the table, pieces of at
-// least 256 keys (a warp's ramp of ~2 us costs as much as ~64 keys a warp) and
-// at most 2048, so that a batch of mixed lengths ends evenly; longer pieces
-// again where a wide table would make more than 65536 CTAs, most of them empty.
-Plan plan_of(int B, int max_q, int H, int H_kv, int bs, int max_blocks) {
+// How a call is cut into CTAs, from its sizes alone (contexts are on the device;
+// `keys`, the table's width, bounds them). A unit is (sequence, KV head, group of
+// 8 NT query rows). Measured on B200, 8 KV heads, G = 4, D = 128, in us.
+//  * NT, the smallest of 1, 2, 4 that holds a KV head's rows, or a smaller one while
+//    its units still leave room on the SMs: a warp with fewer accumulators is
+//    faster, and re-reads come from L2 (16 rows, 8 sequences of 1000 tokens: NT 1
+//    13.3, NT 2 13.8; 16 sequences of 4000: 59.8 and 47.5).
+//  * Contexts are cut while one wave of CTAs has room for the pieces: pieces of one
+//    wave share HBM evenly and end together (8 x 16K-32K, int8: 4096 keys a piece 70,
+//    1024 keys 81), and every CTA pays 3 to 4 us of latencies. A piece is at least
+//    256 keys and at most 1 MB of rows, which a CTA alone on its SM streams in
+//    about 30 us, so one long context in a batch does not outlast the others by
+//    more.
+//  * Pieces of short contexts (a table of at most 2048 keys) with four or more to a
+//    unit are a cluster, else the workspace and the joining kernel hold them (one
+//    sequence of 1000: cluster 7.0, joined 7.8, and 5 us less host time for the
+//    second launch and the workspace; 8 x 4000: 19.0 and 17.6).
+Plan plan_of(int B, int max_q, int H, int H_kv, int D, int fmt, int bs, int max_blocks) {
+  auto round_up = [](int64_t x, int64_t m) { return (x + m - 1) / m * m; };
   Plan r;
   const int rows = max_q * (H / H_kv);
-  r.NT = rows <= 8 ? 1 : rows <= 16 ? 2 : 4;
-  const int64_t units =
-      static_cast<int64_t>(B) * H_kv * ((rows + 8 * r.NT - 1) / (8 * r.NT));
+  const int64_t heads = static_cast<int64_t>(B) * H_kv;
   const int64_t keys = std::max<int64_t>(1, static_cast<int64_t>(max_blocks) * bs);
-  const int64_t slots = static_cast<int64_t>(num_sms()) * (r.NT == 1 ? 3 : 2);
-  const int64_t want = std::max<int64_t>(1, (2 * slots + units - 1) / units);
-  auto round_up = [](int64_t x, int64_t m) { return (x + m - 1) / m * m; };
-  int64_t chunk = round_up((keys + want - 1) / want, 128);
-  chunk = std::min<int64_t>(std::max<int64_t>(chunk, 256), 2048);
+  int64_t units = 0, slots = 0;
+  for (r.NT = 1;; r.NT *= 2) {
+    units = heads * ((rows + 8 * r.NT - 1) / (8 * r.NT));
+    slots = static_cast<int64_t>(num_sms()) * (r.NT == 1 ? 3 : 2);  // resident CTAs
+    if (r.NT == 4 || rows <= 8 * r.NT || (r.NT == 1 ? 2 : 1) * units <= slots) break;
+  }
+  const int64_t per = std::max<int64_t>(1, slots / units);  // pieces of a unit in one wave
+  r.cluster = 1;
+  if (keys <= 2048 && per >= 4)
+    while (r.cluster < 8 && r.cluster * 2 <= per && keys > 128 * r.cluster) r.cluster *= 2;
+  if (r.cluster > 1) {
+    r.nsplit = 1;
+    r.chunk = 0;
+    r.grid = units * r.cluster;
+    return r;
+  }
+  const int64_t cap = (1 << 20) / (2 * D * (fmt == LK_KV_16BIT ? 2 : 1));
+  int64_t chunk = round_up((keys + per - 1) / per, 64);
+  chunk = std::min(std::max<int64_t>(chunk, 256), cap);
+  // a wide table of a large batch: no more than 65536 CTAs, most of them empty
   const int64_t most = std::max<int64_t>(1, 65536 / units);
-  chunk = std::max(chunk, round_up((keys + most - 1) / most, 128));
+  chunk = std::max(chunk, round_up((keys + most - 1) / most, 64));
   r.chunk = static_cast<int>(std::min<int64_t>(chunk, 1 << 30));
   r.nsplit = static_cast<int>((keys + r.chunk - 1) / r.chunk);
   r.grid = units * r.nsplit;
@@ -138,15 +163,28 @@ cudaError_t join(const JoinParams& j, unsigned rows, cudaStream_t s) {
   return launch_after_previous(tree_join_kernel<T, D, 4>, dim3(rows), dim3(128), 0, s, j);
 }
 
+// p.bs_mul / p.bs_shift: exact quotients by bs for keys below 2^31. With
+// l = ceil(log2 bs), m = floor(2^(31 + l) / bs) + 1 < 2^32 exceeds 2^(31 + l) / bs by
+// at most 1, so key m / 2^(31 + l) passes key / bs by less than 1 / bs.
+void set_divisor(TreeParams& p) {
+  int l = 0;
+  while ((1LL << l) < p.bs) ++l;
+  const bool power = (1LL << l) == p.bs;
+  p.bs_mul = power ? 0u : static_cast<uint32_t>((1ull << (31 + l)) / p.bs + 1);
+  p.bs_shift = power ? l : l - 1;
+}
+
 int run(TreeParams& p, int T, int H, int D, float scale, int dtype, int fmt, void* workspace,
         size_t workspace_bytes, cudaStream_t s) {
-  const Plan r = plan_of(p.B, p.max_q, H, p.H_kv, p.bs, p.max_blocks);
+  const Plan r = plan_of(p.B, p.max_q, H, p.H_kv, D, fmt, p.bs, p.max_blocks);
   if (r.grid > 0x7fffffffLL || static_cast<int64_t>(T) * H > 0x7fffffffLL) return LK_ERR_INVALID_ARG;
   const size_t need = plan_bytes(r, T, H, D);
   if (need > 0 && (workspace == nullptr || workspace_bytes < need ||
                    (reinterpret_cast<uintptr_t>(workspace) & 15u) != 0))
     return LK_ERR_WORKSPACE;
+  set_divisor(p);
   p.scale_log2 = scale * 1.4426950408889634f;
+  p.cluster = r.cluster;
   p.chunk = r.chunk;
   p.nsplit = r.nsplit;
   p.part_ml = static_cast<float4*>(workspace);
@@ -200,12 +238,13 @@ bool aligned(const void* a) { return (reinterpret_cast<uintptr_t>(a) & 15u) == 0
 extern "C" size_t lk_paged_tree_workspace_bytes(int32_t num_tokens, int32_t num_seqs,
                                                 int32_t max_q_len, int32_t H, int32_t H_kv,
                                                 int32_t D, int32_t block_size,
-                                                int32_t max_blocks_per_seq) {
+                                                int32_t max_blocks_per_seq, int32_t kv_format) {
   if (num_tokens <= 0 || num_seqs <= 0 || max_q_len <= 0 || H <= 0 || H_kv <= 0 ||
       H % H_kv != 0 || D <= 0 || block_size <= 0 || max_blocks_per_seq <= 0)
     return 0;
   return lk::plan_bytes(
-      lk::plan_of(num_seqs, max_q_len, H, H_kv, block_size, max_blocks_per_seq), num_tokens, H, D);
+      lk::plan_of(num_seqs, max_q_len, H, H_kv, D, kv_format, block_size, max_blocks_per_seq),
+      num_tokens, H, D);
 }
 
 extern "C" int lk_paged_tree_attention(

@@ -28,10 +28,15 @@
 //    1, and the vote costs one instruction where the maximum costs six shuffles).
 //    8-bit caches hold two: m for the sum of p, M for the weights p s_v, which
 //    are rounded to f16 relative to their own maximum. Sums stay in fp32.
-//  * Splits write (m, l, M, O) and a second small kernel joins them; a sequence
-//    that fits one split is written directly.
+//  * Up to eight splits of a context are a thread-block cluster that cuts every
+//    context evenly and joins its (m, l, M, O) over distributed shared memory:
+//    one launch, no workspace. More splits write partials to the workspace and a
+//    second small kernel joins them; a context in one split is written directly.
 #pragma once
 
+#include <cooperative_groups.h>
+
+#include <atomic>
 #include <type_traits>
 
 #include "lk_q8.cuh"
@@ -46,13 +51,16 @@ constexpr float kRaise = 8.f;  // log2 of the largest weight
 template <int FMT, typename T> struct MmaType { using type = __half; };
 template <typename T> struct MmaType<LK_KV_16BIT, T> { using type = T; };
 
-template <int FMT, int D> struct Shape {
+template <int FMT, int D, int NT> struct Shape {
   static constexpr int kEsz = FMT == LK_KV_16BIT ? 2 : 1;
   static constexpr int kRow = D * kEsz;       // bytes of a key row
   static constexpr int kCpr = kRow / 16;      // 16-byte pieces of a row
-  static constexpr int kTok = kEsz == 1 ? 32 : 16;  // keys per stage: 8 KB of K and V at D = 128
+  // Keys per stage and stages per ring: 16 KB of a warp's rows in flight or in use
+  // at D = 128. Two m-tiles per stage share a vote and hide each other's
+  // latency, where the accumulators leave registers for them.
+  static constexpr int kTok = kEsz == 1 && NT == 1 ? 32 : 16;
   static constexpr int kMt = kTok / 16;
-  static constexpr int kNst = 3;
+  static constexpr int kNst = (NT == 1 ? 2 : 3) * (D == 64 ? 2 : 1);
   static constexpr int kTile = kTok * kRow;
   static constexpr int kScales = kEsz == 1 ? 2 * kTok * 4 : 0;
   static constexpr int kStage = 2 * kTile + kScales;
@@ -83,15 +91,17 @@ template <> LK_DEVINL __half round_to<__half>(float x) { return __float2half_rn(
 template <int FMT, typename T, int D, int NT> struct Smem {
   static constexpr int kCols = 8 * NT;
   static constexpr int kQStride = D * 2 + 16;  // bytes; rows shift by 16 bytes: no bank conflicts
-  static constexpr int kMerge = kWarps * kCols * (D + 4) * 4 + kWarps * kCols * 16;
-  static constexpr int kMain = Shape<FMT, D>::kRing > kMerge ? Shape<FMT, D>::kRing : kMerge;
+  // the warps' partials, then the CTA's for its cluster
+  static constexpr int kMerge = (kWarps + 1) * kCols * ((D + 4) * 4 + 16);
+  static constexpr int kRing = Shape<FMT, D, NT>::kRing;
+  static constexpr int kMain = kRing > kMerge ? kRing : kMerge;
   static constexpr int kBytes = kMain + kCols * kQStride + kCols * 12;
 };
 
 template <int FMT, typename T, int D, int NT>
-__global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 2)
+__global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2)
 paged_tree_kernel(const TreeParams p) {
-  using S = Shape<FMT, D>;
+  using S = Shape<FMT, D, NT>;
   using SM = Smem<FMT, T, D, NT>;
   using MT = typename MmaType<FMT, T>::type;
   constexpr bool Q8B = FMT != LK_KV_16BIT;
@@ -110,12 +120,27 @@ paged_tree_kernel(const TreeParams p) {
 
   const int col_groups = (p.max_q * p.G + COLS - 1) / COLS;
   unsigned u = blockIdx.x;
+  int sp = 0;
+  if (p.cluster > 1) {
+    sp = u % p.cluster;
+    u /= p.cluster;
+  }
   const int cg = u % col_groups;
   u /= col_groups;
   const int kvh = u % p.H_kv;
   u /= p.H_kv;
   const int b = u % p.B;
-  const int sp = u / p.B;
+  if (p.cluster == 1) sp = u / p.B;
+  auto quotient = [&](int key) {
+    return static_cast<int>(p.bs_mul ? __umulhi(key, p.bs_mul) >> p.bs_shift
+                                     : static_cast<uint32_t>(key) >> p.bs_shift);
+  };
+  const int32_t* bt = p.block_tables + static_cast<int64_t>(b) * p.bt_stride;
+  // Where the split's start does not depend on the context's length, the first
+  // stage's block is read beside that length, not after it.
+  int early = 0;
+  if (p.cluster == 1)
+    early = __ldg(bt + min(quotient(sp * p.chunk + warp * S::kTok + lane), p.max_blocks - 1));
 
   int row0 = b, n = 1;
   if (p.cu_seqlens_q) {
@@ -133,17 +158,21 @@ paged_tree_kernel(const TreeParams p) {
     if (threadIdx.x == 0 && p.status) atomicOr(p.status, LK_STATUS_CTX_OOB);
     ctx = max(min(ctx, p.max_blocks * p.bs), 0);
   }
-  const int key0 = sp * p.chunk;
-  if (key0 >= ctx && sp > 0) return;
-  const int key1 = min(ctx, key0 + p.chunk);
+  // A cluster cuts every context into even pieces; its CTAs all stay.
+  const int chunk =
+      p.cluster > 1 ? ((ctx + S::kTok - 1) / S::kTok + p.cluster - 1) / p.cluster * S::kTok
+                    : p.chunk;
+  const int key0 = min(sp * chunk, ctx);
+  if (p.cluster == 1 && sp * chunk >= ctx && sp > 0) return;
+  const int key1 = min(ctx, key0 + chunk);
   // keys below `open` are seen by every row
   const int open = p.cu_seqlens_q ? max(ctx - n, 0) : ctx;
 
   // ------------------------------------------------------------ the ring ---
-  const int64_t width = static_cast<int64_t>(p.H_kv) * S::kRow;  // bytes of a slot
-  const uint8_t* kbase = static_cast<const uint8_t*>(p.k) + kvh * S::kRow;
-  const uint8_t* vbase = static_cast<const uint8_t*>(p.v) + kvh * S::kRow;
-  const int32_t* bt = p.block_tables + static_cast<int64_t>(b) * p.bt_stride;
+  const uint32_t width = p.H_kv * S::kRow;  // bytes of a slot
+  const int pc = lane % S::kCpr;            // the lane's piece of the rows it copies
+  const uint8_t* kbase = static_cast<const uint8_t*>(p.k) + kvh * S::kRow + pc * 16;
+  const uint8_t* vbase = static_cast<const uint8_t*>(p.v) + kvh * S::kRow + pc * 16;
   uint8_t* ring = smem + warp * (S::kNst * S::kStage);
   const int nstage = (key1 - key0 + S::kTok - 1) / S::kTok;
   const int mine = nstage > warp ? (nstage - warp + kWarps - 1) / kWarps : 0;
@@ -152,7 +181,7 @@ paged_tree_kernel(const TreeParams p) {
   auto block_of = [&](int i) {
     const int key = first_key(i) + lane;
     if (i >= mine || lane >= S::kTok || key >= key1) return -1;
-    const int blk = __ldg(bt + key / p.bs);
+    const int blk = i == 0 && p.cluster == 1 ? early : __ldg(bt + quotient(key));
     if (blk < 0 || blk >= p.num_blocks) {
       if (p.status) atomicOr(p.status, LK_STATUS_BLOCK_OOB);
       return -1;
@@ -161,24 +190,26 @@ paged_tree_kernel(const TreeParams p) {
   };
   auto load_stage = [&](int i, int blk) {
     uint8_t* st = ring + (i % S::kNst) * S::kStage;
-    const int off = (first_key(i) + lane) % p.bs;
+    const int key = first_key(i) + lane;
+    const int off = key - quotient(key) * p.bs;
     const int slot = blk < 0 ? -1 : blk * p.bs + off;
     constexpr int RPI = 32 / S::kCpr;  // rows per copy instruction
-    const int pc = lane % S::kCpr;
 #pragma unroll
     for (int j = 0; j < S::kTok / RPI; ++j) {
       const int r = j * RPI + lane / S::kCpr;
       const int sl = __shfl_sync(0xffffffffu, slot, r);
-      const int64_t at = sl < 0 ? 0 : sl * width + pc * 16;
+      const uint64_t at = static_cast<uint64_t>(static_cast<uint32_t>(max(sl, 0))) * width;
       const uint32_t to = piece<S::kCpr>(r, pc);
       cp_async16(st + to, kbase + at, sl >= 0);
       cp_async16(st + S::kTile + to, vbase + at, sl >= 0);
     }
     if constexpr (Q8B) {
-      float* sc = reinterpret_cast<float*>(st + 2 * S::kTile);
-      const int64_t at = slot < 0 ? 0 : (static_cast<int64_t>(blk) * p.H_kv + kvh) * p.bs + off;
-      cp_async4(sc + lane, p.k_scale + at, slot >= 0);
-      cp_async4(sc + S::kTok + lane, p.v_scale + at, slot >= 0);
+      if (lane < S::kTok) {
+        float* sc = reinterpret_cast<float*>(st + 2 * S::kTile);
+        const int64_t at = slot < 0 ? 0 : (static_cast<int64_t>(blk) * p.H_kv + kvh) * p.bs + off;
+        cp_async4(sc + lane, p.k_scale + at, slot >= 0);
+        cp_async4(sc + S::kTok + lane, p.v_scale + at, slot >= 0);
+      }
     }
   };
   int next = block_of(0);
@@ -259,13 +290,13 @@ paged_tree_kernel(const TreeParams p) {
     for (int nt = 0; nt < NT; ++nt) o[i][nt][0] = o[i][nt][1] = o[i][nt][2] = o[i][nt][3] = 0.f;
   // Start of the running maxima: finite, so that a masked score (-inf) less it
   // is -inf and never NaN.
-  float m[NT][2], l[NT][2], M[NT][2];
+  float m[NT][2], l[NT][2], M[NT][2], dm[NT][2];  // dm = m - M
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       m[nt][h] = M[nt][h] = -3.402823466e38f;
-      l[nt][h] = 0.f;
+      l[nt][h] = dm[nt][h] = 0.f;
     }
 
   // Which of the keys t0 .. t0 + 31 column j sees, one bit each: all below
@@ -360,9 +391,12 @@ paged_tree_kernel(const TreeParams p) {
       }
     }
 
-    // scores in base 2; elements 0, 1: key g, columns 2c, 2c + 1; 2, 3: key g + 8
+    // Scores in base 2, less the running maxima: elements 0, 1 are key g and
+    // columns 2c, 2c + 1; elements 2, 3 key g + 8.
     const int t0 = first_key(i);
-    float lsv[S::kMt][2];
+    const bool drafts = min(t0 + S::kTok, key1) > open;
+    const bool masked = t0 + S::kTok > key1 || drafts;
+    float f[S::kMt][NT][4], lsv[S::kMt][2];
 #pragma unroll
     for (int mt = 0; mt < S::kMt; ++mt) {
       float s0 = 1.f, s1 = 1.f;
@@ -374,50 +408,65 @@ paged_tree_kernel(const TreeParams p) {
       }
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        x[mt][nt][0] = x[mt][nt][0] * s0 * cs[nt][0];
-        x[mt][nt][1] = x[mt][nt][1] * s0 * cs[nt][1];
-        x[mt][nt][2] = x[mt][nt][2] * s1 * cs[nt][0];
-        x[mt][nt][3] = x[mt][nt][3] * s1 * cs[nt][1];
+        f[mt][nt][0] = s0 * cs[nt][0];
+        f[mt][nt][1] = s0 * cs[nt][1];
+        f[mt][nt][2] = s1 * cs[nt][0];
+        f[mt][nt][3] = s1 * cs[nt][1];
       }
     }
-    const bool drafts = min(t0 + S::kTok, key1) > open;
-    if (t0 + S::kTok > key1 || drafts) {
+    if (masked) {
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const uint32_t bits = window(nt * 8 + 2 * c + h, t0) >> g;
 #pragma unroll
-          for (int mt = 0; mt < S::kMt; ++mt) {
-            if (!((bits >> (mt * 16)) & 1u)) x[mt][nt][h] = -INFINITY;
-            if (!((bits >> (mt * 16 + 8)) & 1u)) x[mt][nt][2 + h] = -INFINITY;
-          }
+          for (int mt = 0; mt < S::kMt; ++mt)
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              const int e = 2 * k + h;
+              x[mt][nt][e] = (bits >> (mt * 16 + 8 * k)) & 1u ? x[mt][nt][e] * f[mt][nt][e]
+                                                              : -INFINITY;
+              f[mt][nt][e] = 1.f;
+            }
         }
     }
-
-    // raise the maxima when a score passes them by more than kRaise
-    bool up = false;
+    float d[S::kMt][NT][4], d2[S::kMt][NT][4];
+    auto scores = [&]() {
+      float top = -INFINITY;
 #pragma unroll
-    for (int mt = 0; mt < S::kMt; ++mt)
+      for (int mt = 0; mt < S::kMt; ++mt)
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          up |= x[mt][nt][e] - m[nt][e & 1] > kRaise;
-          if constexpr (Q8B) up |= x[mt][nt][e] + lsv[mt][e >> 1] - M[nt][e & 1] > kRaise;
-        }
-    if (__any_sync(0xffffffffu, up)) {
+          for (int e = 0; e < 4; ++e) {
+            d[mt][nt][e] = fmaf(x[mt][nt][e], f[mt][nt][e], -m[nt][e & 1]);
+            if constexpr (Q8B) {
+              d2[mt][nt][e] = d[mt][nt][e] + (lsv[mt][e >> 1] + dm[nt][e & 1]);
+              // a masked weight is zero even where its row's scale is NaN
+              if (masked && d[mt][nt][e] == -INFINITY) d2[mt][nt][e] = -INFINITY;
+              top = fmax3(top, d[mt][nt][e], d2[mt][nt][e]);
+            } else {
+              top = fmaxf(top, d[mt][nt][e]);
+            }
+          }
+      return top;
+    };
+    // raise the maxima where a weight would pass 2^kRaise
+    if (__any_sync(0xffffffffu, scores() > kRaise)) {
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           float a = m[nt][h], w = M[nt][h];
 #pragma unroll
-          for (int mt = 0; mt < S::kMt; ++mt) {
-            a = fmaxf(a, fmaxf(x[mt][nt][h], x[mt][nt][2 + h]));
-            if constexpr (Q8B)
-              w = fmaxf(w, fmaxf(x[mt][nt][h] + lsv[mt][0], x[mt][nt][2 + h] + lsv[mt][1]));
-          }
+          for (int mt = 0; mt < S::kMt; ++mt)
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              const float y = x[mt][nt][2 * k + h] * f[mt][nt][2 * k + h];
+              a = fmaxf(a, y);
+              if constexpr (Q8B) w = fmaxf(w, y == -INFINITY ? y : y + lsv[mt][k]);
+            }
 #pragma unroll
           for (int off = 4; off < 32; off <<= 1) {
             a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, off));
@@ -428,12 +477,14 @@ paged_tree_kernel(const TreeParams p) {
           const float al = ex2_mufu(M[nt][h] - w);
           m[nt][h] = a;
           M[nt][h] = w;
+          if constexpr (Q8B) dm[nt][h] = a - w;
 #pragma unroll
           for (int k = 0; k < KS; ++k) {
             o[k][nt][h] *= al;
             o[k][nt][2 + h] *= al;
           }
         }
+      scores();
     }
 
     // weights
@@ -445,13 +496,9 @@ paged_tree_kernel(const TreeParams p) {
         float w[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          w[e] = ex2_mufu(x[mt][nt][e] - m[nt][e & 1]);
+          w[e] = ex2_mufu(d[mt][nt][e]);
           l[nt][e & 1] += w[e];
-          if constexpr (Q8B) {
-            const float y = x[mt][nt][e];
-            // a masked weight is zero even where the row's scale is NaN
-            w[e] = y == -INFINITY ? 0.f : ex2_mufu(y + lsv[mt][e >> 1] - M[nt][e & 1]);
-          }
+          if constexpr (Q8B) w[e] = ex2_mufu(d2[mt][nt][e]);
         }
         pb[mt][nt][0] = pack2<MT>(w[0], w[1]);
         pb[mt][nt][1] = pack2<MT>(w[2], w[3]);
@@ -573,7 +620,11 @@ paged_tree_kernel(const TreeParams p) {
         pm[warp * COLS + col] = make_float4(m[nt][h], l[nt][h], Q8B ? M[nt][h] : m[nt][h], 0.f);
     }
   __syncthreads();
-  const bool whole = key0 == 0 && key1 == ctx;  // one split holds the whole context
+  const int H = p.H_kv * p.G;
+  const bool whole = p.cluster == 1 && key0 == 0 && key1 == ctx;
+  // the CTA's own partials, for its cluster: [col][OS], [col]
+  float* co = reinterpret_cast<float*>(pm + kWarps * COLS);
+  float4* cm = reinterpret_cast<float4*>(co + COLS * OS);
   for (int j = warp; j < COLS; j += kWarps) {
     const int token = col_token[j];
     if (token < 0) continue;
@@ -594,7 +645,7 @@ paged_tree_kernel(const TreeParams p) {
     const int64_t row = static_cast<int64_t>(row0 + token);
     // no visible key: L = 0 and the row is 0 / 0 = NaN
     const float fin = (Q8B ? exp2f(A - a) : 1.f) / L;
-    const int64_t part = (row * (p.H_kv * p.G) + col_head[j]) * p.nsplit + sp;
+    const int64_t part = (row * H + col_head[j]) * p.nsplit + sp;
 #pragma unroll
     for (int i = 0; i < D / 32; ++i) {
       const int d = lane + 32 * i;
@@ -602,25 +653,85 @@ paged_tree_kernel(const TreeParams p) {
 #pragma unroll
       for (int t = 0; t < kWarps; ++t) acc += po[(t * COLS + j) * OS + d] * f[t];
       if (whole)
-        static_cast<T*>(p.out)[row * p.out_stride + col_head[j] * D + d] =
-            round_to<T>(acc * fin);
+        static_cast<T*>(p.out)[row * p.out_stride + col_head[j] * D + d] = round_to<T>(acc * fin);
+      else if (p.cluster > 1)
+        co[j * OS + d] = acc;
       else
         p.part_o[part * D + d] = acc;
     }
-    if (!whole && lane == 0) p.part_ml[part] = make_float4(a, L, A, 0.f);
+    if (!whole && lane == 0)
+      *(p.cluster > 1 ? cm + j : p.part_ml + part) = make_float4(a, L, A, 0.f);
   }
+  if (p.cluster == 1) return;
+
+  // ------------------------------------------------------ join the cluster ---
+  // CTA r of the cluster joins columns r, r + n, ..., in split order.
+  namespace cg_ = cooperative_groups;
+  cg_::cluster_group cluster = cg_::this_cluster();
+  cluster.sync();
+  const int n_cta = min(p.cluster, max(1, (ctx + chunk - 1) / max(chunk, 1)));  // that held keys
+  for (int j = sp + warp * p.cluster; j < COLS; j += kWarps * p.cluster) {
+    const int token = col_token[j];
+    if (token < 0) continue;
+    float a = -3.402823466e38f, A = a;
+    for (int i = 0; i < n_cta; ++i) {
+      const float4 w = *cluster.map_shared_rank(cm + j, i);
+      a = fmaxf(a, w.x);
+      A = fmaxf(A, w.z);
+    }
+    float L = 0.f, acc[D / 32];
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) acc[i] = 0.f;
+#pragma unroll 4
+    for (int i = 0; i < n_cta; ++i) {
+      const float4 w = *cluster.map_shared_rank(cm + j, i);
+      const float* src = cluster.map_shared_rank(co + j * OS, i);
+      const float f = ex2_mufu(w.z - A);
+      L += w.y * ex2_mufu(w.x - a);
+#pragma unroll
+      for (int k = 0; k < D / 32; ++k) acc[k] += src[lane + 32 * k] * f;
+    }
+    const float fin = (Q8B ? exp2f(A - a) : 1.f) / L;
+    T* dst = static_cast<T*>(p.out) + static_cast<int64_t>(row0 + token) * p.out_stride +
+             col_head[j] * D;
+#pragma unroll
+    for (int k = 0; k < D / 32; ++k) dst[lane + 32 * k] = round_to<T>(acc[k] * fin);
+  }
+  cluster.sync();  // no CTA leaves while another reads its partials
 }
 
 template <int FMT, typename T, int D, int NT>
 int launch(const TreeParams& p, unsigned grid, cudaStream_t s) {
   constexpr int bytes = Smem<FMT, T, D, NT>::kBytes;
   auto* kernel = paged_tree_kernel<FMT, T, D, NT>;
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) !=
-      cudaSuccess)
-    return LK_ERR_CUDA;
-  if (launch_after_previous(kernel, dim3(grid), dim3(kWarps * 32), bytes, s, p) != cudaSuccess)
-    return LK_ERR_CUDA;
-  return check_launch();
+  static std::atomic<uint64_t> ready{0};  // devices whose function attribute is set
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return LK_ERR_CUDA;
+  const uint64_t bit = 1ull << (dev & 63);
+  if (!(ready.load(std::memory_order_relaxed) & bit)) {
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) !=
+        cudaSuccess)
+      return LK_ERR_CUDA;
+    if (dev < 64) ready.fetch_or(bit, std::memory_order_relaxed);
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(kWarps * 32);
+  cfg.dynamicSmemBytes = bytes;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  if (pdl_enabled()) {
+    attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
+  }
+  if (p.cluster > 1) {
+    attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+    attr[cfg.numAttrs].val.clusterDim.x = p.cluster;
+    attr[cfg.numAttrs].val.clusterDim.y = 1;
+    attr[cfg.numAttrs++].val.clusterDim.z = 1;
+  }
+  cfg.attrs = attr;
+  return cudaLaunchKernelEx(&cfg, kernel, p) == cudaSuccess ? check_launch() : LK_ERR_CUDA;
 }
 
 template <int FMT, typename T, int D>

@@ -26,10 +26,13 @@ struct TreeParams {
   int32_t* status;
   int T;                        // rows of q and out
   int B, H_kv, G, bs, max_blocks;
+  uint32_t bs_mul;              // key / bs: key >> bs_shift if 0, else umulhi(key, bs_mul) >> bs_shift
+  int bs_shift;
   int64_t num_blocks;
   int max_q;                    // most query tokens of a sequence
   float scale_log2;             // scale * log2(e)
-  int chunk;                    // keys per split, a multiple of 64
+  int cluster;                  // > 1: a unit's splits are one cluster of that many CTAs
+  int chunk;                    // keys per split (cluster: set by each context)
   int nsplit;                   // 1: every CTA writes out itself
   float4* part_ml;              // [T * H][nsplit]: m, l, M, unused
   float* part_o;                // [T * H][nsplit][D]

@@ -27,15 +27,16 @@ def _dtype_code(t: torch.Tensor, allowed=(torch.float16, torch.bfloat16)) -> int
 
 
 def _cuda(*ts: Optional[torch.Tensor]) -> torch.device:
-    dev = None
+    dev, index = None, -1
     for t in ts:
         if t is None:
             continue
-        if not t.is_cuda:
+        i = t.get_device()
+        if i < 0:
             raise RuntimeError("litevllm_b200 kernels run on CUDA tensors only (no CPU fallback)")
         if dev is None:
-            dev = t.device
-        elif t.device != dev:
+            dev, index = t.device, i
+        elif i != index:
             raise RuntimeError(f"tensors on different devices: {dev} vs {t.device}")
     assert dev is not None
     return dev
@@ -46,7 +47,9 @@ def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
 
 
 def _stream(dev: torch.device) -> int:
-    return torch.cuda.current_stream(dev).cuda_stream
+    # the handle alone: building a torch.cuda.Stream object costs 2.5 us a call
+    return torch._C._cuda_getCurrentRawStream(
+        torch.cuda.current_device() if dev.index is None else dev.index)
 
 
 _NULL = contextlib.nullcontext()
@@ -273,17 +276,17 @@ def load_kvcache_q8(
     return tuple(outs)
 
 
-def _tree_workspace(dev, workspace, T, B, max_q, H, H_kv, D, bs, max_blocks):
+def _tree_workspace(dev, workspace, T, B, max_q, H, H_kv, D, bs, max_blocks, fmt):
     """(pointer, bytes, tensor to keep alive). Without a caller's workspace the
     partials of split contexts live in a buffer of this call's own, from torch's
     allocator: calls on other streams and captured graphs never share it."""
-    key = (dev.index, T, B, max_q, H, H_kv, D, bs, max_blocks)
+    key = (dev.index, T, B, max_q, H, H_kv, D, bs, max_blocks, fmt)
     need = _TREE_WS.get(key)
     if need is None:
         if len(_TREE_WS) > 65536:  # token counts vary from step to step
             _TREE_WS.clear()
         need = _TREE_WS[key] = int(lib().lk_paged_tree_workspace_bytes(
-            T, B, max_q, H, H_kv, D, bs, max_blocks))
+            T, B, max_q, H, H_kv, D, bs, max_blocks, fmt))
     if workspace is None:
         if need == 0:
             return None, 0, None
@@ -298,11 +301,13 @@ _TREE_WS: dict = {}  # shape -> lk_paged_tree_workspace_bytes, asked once per sh
 
 
 def tree_workspace_bytes(num_tokens: int, num_seqs: int, max_q_len: int, H: int, H_kv: int,
-                         D: int, block_size: int, max_blocks: int) -> int:
+                         D: int, block_size: int, max_blocks: int,
+                         cache_dtype: torch.dtype = torch.bfloat16) -> int:
     """Bytes of a caller-owned workspace for paged_tree_attention (decode:
     num_tokens = num_seqs and max_q_len = 1), of the current device."""
-    return int(lib().lk_paged_tree_workspace_bytes(num_tokens, num_seqs, max_q_len, H, H_kv, D,
-                                                   block_size, max_blocks))
+    return int(lib().lk_paged_tree_workspace_bytes(
+        num_tokens, num_seqs, max_q_len, H, H_kv, D, block_size, max_blocks,
+        _KV_FORMATS.get(cache_dtype, LK_KV_16BIT)))
 
 
 def paged_decode_q8(
@@ -407,7 +412,8 @@ def _tree(dev, query, kd, ks, vd, vs, fmt, block_tables, context_lens, cu, mask,
     if T == 0 or B == 0 or max_q == 0:
         return out
     with _on(dev):
-        ws, ws_bytes, keep = _tree_workspace(dev, workspace, T, B, max_q, H, H_kv, D, bs, max_blocks)
+        ws, ws_bytes, keep = _tree_workspace(dev, workspace, T, B, max_q, H, H_kv, D, bs,
+                                             max_blocks, fmt)
         args = (B, H, H_kv, D, bs, max_blocks, float(scale), code, fmt, ws, ws_bytes, _ptr(status),
                 _stream(dev))
         head = (out.data_ptr(), out.stride(0), query.data_ptr(), query.stride(0), kd.data_ptr(),

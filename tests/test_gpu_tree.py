@@ -214,8 +214,8 @@ def test_streams_and_graphs_do_not_share_state(cuda, kind):
 
 
 def test_caller_owned_workspace(cuda):
-    c = case(INT8, BF16, 8, 2, 128, 16, [3000, 20], [4, 4], seed=12)
-    need = ops.tree_workspace_bytes(8, 2, 4, 8, 2, 128, 16, c["tables"].shape[1])
+    c = case(INT8, BF16, 8, 2, 128, 16, [9000, 20], [4, 4], seed=12)
+    need = ops.tree_workspace_bytes(8, 2, 4, 8, 2, 128, 16, c["tables"].shape[1], INT8)
     assert need > 0
     got = run(c, cuda, workspace=torch.empty(need, dtype=torch.uint8, device=cuda))
     assert torch.equal(got, run(c, cuda))

@@ -73,7 +73,7 @@ def test_tree_rejects_bad_arguments():
     assert f(*replaced(args, _4=P + 4)) == -3
     # a table that is split wants its workspace
     wide = replaced(args, _23=4096)
-    need = _lib.lib().lk_paged_tree_workspace_bytes(8, 2, 4, 32, 8, 128, 16, 4096)
+    need = _lib.lib().lk_paged_tree_workspace_bytes(8, 2, 4, 32, 8, 128, 16, 4096, 1)
     assert need > 0
     assert f(*replaced(wide, _27=None, _28=0)) == -4
     assert f(*replaced(wide, _28=need - 1)) == -4
@@ -89,10 +89,10 @@ def test_tree_rejects_bad_arguments():
 
 def test_tree_workspace_sizes():
     f = _lib.lib().lk_paged_tree_workspace_bytes
-    assert f(8, 8, 1, 32, 8, 128, 16, 8) == 0               # 128 keys: no split
-    assert f(0, 8, 1, 32, 8, 128, 16, 8) == 0
-    assert f(8, 8, 1, 32, 7, 128, 16, 8) == 0
-    one = f(1, 1, 1, 32, 8, 128, 16, 8192)
+    assert f(8, 8, 1, 32, 8, 128, 16, 8, 1) == 0               # 128 keys: no split
+    assert f(0, 8, 1, 32, 8, 128, 16, 8, 1) == 0
+    assert f(8, 8, 1, 32, 7, 128, 16, 8, 1) == 0
+    one = f(1, 1, 1, 32, 8, 128, 16, 8192, 1)
     assert one % (32 * (128 + 4) * 4) == 0 and one > 0
 
 

@@ -78,6 +78,37 @@ int load_encode() {
 
 }  // namespace
 
+int make_kv_tensor_map(CUtensorMap* out, const void* base, int64_t num_slots, int H_kv, int D,
+                       int dtype, int box_slots, int box_heads) {
+  const bool bytes = dtype == kMapBytes;
+  if (dtype != LK_DTYPE_BF16 && dtype != LK_DTYPE_F16 && !bytes) return LK_ERR_UNSUPPORTED;
+  if ((reinterpret_cast<uintptr_t>(base) & 15u) != 0) return LK_ERR_ALIGNMENT;
+  {
+    std::lock_guard<std::mutex> lock(g_map_mu);
+    const int rc = load_encode();
+    if (rc != LK_OK) return rc;
+  }
+  const uint64_t esz = bytes ? 1 : 2;
+  // dims: (d, slot, head); the slot stride exceeds the head stride, which
+  // is what puts each head's rows contiguously in shared memory.
+  cuuint64_t dims[3] = {static_cast<cuuint64_t>(D), static_cast<cuuint64_t>(num_slots),
+                        static_cast<cuuint64_t>(H_kv)};
+  cuuint64_t strides[2] = {static_cast<cuuint64_t>(H_kv) * D * esz,
+                           static_cast<cuuint64_t>(D) * esz};
+  cuuint32_t box[3] = {bytes ? static_cast<cuuint32_t>(D) : 64u,
+                       static_cast<cuuint32_t>(box_slots), static_cast<cuuint32_t>(box_heads)};
+  cuuint32_t estr[3] = {1u, 1u, 1u};
+  CUresult r = g_encode(out,
+                        bytes                    ? CU_TENSOR_MAP_DATA_TYPE_UINT8
+                        : dtype == LK_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+                        3, const_cast<void*>(base), dims, strides, box, estr,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        bytes ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B,
+                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? LK_OK : LK_ERR_DRIVER;
+}
+
 int get_kv_tensor_map(CUtensorMap* out, const void* base, int64_t num_slots, int H_kv, int D,
                       int dtype, int box_slots, int box_heads) {
   if (dtype != LK_DTYPE_BF16 && dtype != LK_DTYPE_F16) return LK_ERR_UNSUPPORTED;
@@ -85,32 +116,18 @@ int get_kv_tensor_map(CUtensorMap* out, const void* base, int64_t num_slots, int
   int dev = 0;
   cudaGetDevice(&dev);
   MapKey key{base, num_slots, H_kv, D, dtype, box_slots, box_heads, dev};
-  std::lock_guard<std::mutex> lock(g_map_mu);
-  auto it = g_maps.find(key);
-  if (it != g_maps.end()) {
-    *out = it->second;
-    return LK_OK;
+  {
+    std::lock_guard<std::mutex> lock(g_map_mu);
+    auto it = g_maps.find(key);
+    if (it != g_maps.end()) {
+      *out = it->second;
+      return LK_OK;
+    }
   }
-  int rc = load_encode();
-  if (rc != LK_OK) return rc;
-  const uint64_t esz = 2;
-  // dims: (d, slot, head); the slot stride exceeds the head stride, which
-  // is what puts each head's rows contiguously in shared memory.
-  cuuint64_t dims[3] = {static_cast<cuuint64_t>(D), static_cast<cuuint64_t>(num_slots),
-                        static_cast<cuuint64_t>(H_kv)};
-  cuuint64_t strides[2] = {static_cast<cuuint64_t>(H_kv) * D * esz,
-                           static_cast<cuuint64_t>(D) * esz};
-  cuuint32_t box[3] = {64u, static_cast<cuuint32_t>(box_slots),
-                       static_cast<cuuint32_t>(box_heads)};
-  cuuint32_t estr[3] = {1u, 1u, 1u};
   CUtensorMap map;
-  CUresult r = g_encode(&map,
-                        dtype == LK_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
-                                               : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
-                        3, const_cast<void*>(base), dims, strides, box, estr,
-                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r != CUDA_SUCCESS) return LK_ERR_DRIVER;
+  const int rc = make_kv_tensor_map(&map, base, num_slots, H_kv, D, dtype, box_slots, box_heads);
+  if (rc != LK_OK) return rc;
+  std::lock_guard<std::mutex> lock(g_map_mu);
   if (g_maps.size() > 4096) g_maps.clear();
   g_maps.emplace(key, map);
   *out = map;

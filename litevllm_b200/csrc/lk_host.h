@@ -27,6 +27,12 @@ int check_launch();
 int get_kv_tensor_map(CUtensorMap* out, const void* base, int64_t num_slots, int H_kv, int D,
                       int dtype, int box_slots, int box_heads);
 
+// The same map encoded for this call, not kept. With dtype kMapBytes the cache
+// holds bytes: one box is box_heads x box_slots x D bytes, unswizzled.
+constexpr int kMapBytes = 16;
+int make_kv_tensor_map(CUtensorMap* out, const void* base, int64_t num_slots, int H_kv, int D,
+                       int dtype, int box_slots, int box_heads);
+
 inline int dtype_size(int dtype) { return dtype == LK_DTYPE_F32 ? 4 : 2; }
 
 // Programmatic dependent launch on (LITEKERN_PDL=0 turns it off; read once).

@@ -97,42 +97,53 @@ __global__ void __launch_bounds__(W * 32) tree_join_kernel(const JoinParams p) {
 }
 
 struct Plan {
-  int NT, cluster, chunk, nsplit;
+  int NT, cluster, chunk, nsplit;  // NT 0: the tcgen05 kernel
   int64_t grid;
 };
 
 // How a call is cut into CTAs, from its sizes alone (contexts are on the device;
 // `keys`, the table's width, bounds them). A unit is (sequence, KV head, group of
-// 8 NT query rows). Measured on B200, 8 KV heads, G = 4, D = 128, in us.
-//  * NT, the smallest of 1, 2, 4 that holds a KV head's rows, or a smaller one while
-//    its units still leave room on the SMs: a warp with fewer accumulators is
-//    faster, and re-reads come from L2 (16 rows, 8 sequences of 1000 tokens: NT 1
-//    13.3, NT 2 13.8; 16 sequences of 4000: 59.8 and 47.5).
+// query rows). Measured on B200, 8 KV heads, G = 4, D = 128, graph-replayed, in us.
+//  * The tcgen05 kernel (128 rows a CTA) where a key row meets enough query rows,
+//    more than 16 of a 16-bit cache or 32 of an 8-bit one (32 rows, 32 x 1000: 16-bit
+//    29 and 35 on mma.sync, int8 41 and 35), and the whole call outweighs its longer
+//    set-up (128 rows, 1 x 4000: 19 and 25; 256 rows, 1 x 256: 15 and 9). Its TMA
+//    boxes want block sizes that are multiples of 16.
+//  * Else NT, the smallest of 1, 2, 4 whose 8 NT rows hold a KV head's, or a smaller
+//    one while its units still leave room on the SMs: a warp with fewer accumulators
+//    is faster, and re-reads come from L2 (16 rows, 8 x 1000: NT 1 13.3, NT 2 13.8;
+//    16 x 4000: 59.8 and 47.5).
 //  * Contexts are cut while one wave of CTAs has room for the pieces: pieces of one
-//    wave share HBM evenly and end together (8 x 16K-32K, int8: 4096 keys a piece 70,
-//    1024 keys 81), and every CTA pays 3 to 4 us of latencies. A piece is at least
-//    256 keys and at most 1 MB of rows, which a CTA alone on its SM streams in
-//    about 30 us, so one long context in a batch does not outlast the others by
-//    more.
+//    wave share HBM evenly and end together (decode, 8 x 16K-32K, int8: 4096 keys a
+//    piece 70, 1024 keys 81), and every CTA pays 3 to 4 us of latencies. A piece is at
+//    least 256 keys and at most 1 MB of rows, which a CTA alone on its SM streams in
+//    about 30 us (tcgen05: 2048 keys), so that one long context in a batch does not
+//    outlast the others by more (64 nodes, 16 x 1K-8K, int8: 258, uncut 288).
 //  * Pieces of short contexts (a table of at most 2048 keys) with four or more to a
-//    unit are a cluster, else the workspace and the joining kernel hold them (one
-//    sequence of 1000: cluster 7.0, joined 7.8, and 5 us less host time for the
-//    second launch and the workspace; 8 x 4000: 19.0 and 17.6).
+//    unit are a cluster, else the workspace and the joining kernel hold them (decode,
+//    1 x 1000: cluster 7.0, joined 7.8, and 5 us less host time for the second launch
+//    and the workspace; 8 x 4000: 19.0 and 17.6).
 Plan plan_of(int B, int max_q, int H, int H_kv, int D, int fmt, int bs, int max_blocks) {
   auto round_up = [](int64_t x, int64_t m) { return (x + m - 1) / m * m; };
   Plan r;
-  const int rows = max_q * (H / H_kv);
+  const int64_t rows = static_cast<int64_t>(max_q) * (H / H_kv);
   const int64_t heads = static_cast<int64_t>(B) * H_kv;
   const int64_t keys = std::max<int64_t>(1, static_cast<int64_t>(max_blocks) * bs);
-  int64_t units = 0, slots = 0;
-  for (r.NT = 1;; r.NT *= 2) {
-    units = heads * ((rows + 8 * r.NT - 1) / (8 * r.NT));
-    slots = static_cast<int64_t>(num_sms()) * (r.NT == 1 ? 3 : 2);  // resident CTAs
-    if (r.NT == 4 || rows <= 8 * r.NT || (r.NT == 1 ? 2 : 1) * units <= slots) break;
+  int64_t units = 0, slots = 0;  // resident CTAs
+  if (rows > (fmt == LK_KV_16BIT ? 16 : 32) && bs % 16 == 0 && heads * keys * rows >= (2 << 20)) {
+    r.NT = 0;
+    units = heads * ((rows + 127) / 128);
+    slots = 2 * num_sms();
+  } else {
+    for (r.NT = 1;; r.NT *= 2) {
+      units = heads * ((rows + 8 * r.NT - 1) / (8 * r.NT));
+      slots = static_cast<int64_t>(num_sms()) * (r.NT == 1 ? 3 : 2);
+      if (r.NT == 4 || rows <= 8 * r.NT || (r.NT == 1 ? 2 : 1) * units <= slots) break;
+    }
   }
   const int64_t per = std::max<int64_t>(1, slots / units);  // pieces of a unit in one wave
   r.cluster = 1;
-  if (keys <= 2048 && per >= 4)
+  if (r.NT > 0 && keys <= 2048 && per >= 4)
     while (r.cluster < 8 && r.cluster * 2 <= per && keys > 128 * r.cluster) r.cluster *= 2;
   if (r.cluster > 1) {
     r.nsplit = 1;
@@ -140,7 +151,7 @@ Plan plan_of(int B, int max_q, int H, int H_kv, int D, int fmt, int bs, int max_
     r.grid = units * r.cluster;
     return r;
   }
-  const int64_t cap = (1 << 20) / (2 * D * (fmt == LK_KV_16BIT ? 2 : 1));
+  const int64_t cap = r.NT == 0 ? 2048 : (1 << 20) / (2 * D * (fmt == LK_KV_16BIT ? 2 : 1));
   int64_t chunk = round_up((keys + per - 1) / per, 64);
   chunk = std::min(std::max<int64_t>(chunk, 256), cap);
   // a wide table of a large batch: no more than 65536 CTAs, most of them empty
@@ -163,15 +174,15 @@ cudaError_t join(const JoinParams& j, unsigned rows, cudaStream_t s) {
   return launch_after_previous(tree_join_kernel<T, D, 4>, dim3(rows), dim3(128), 0, s, j);
 }
 
-// p.bs_mul / p.bs_shift: exact quotients by bs for keys below 2^31. With
-// l = ceil(log2 bs), m = floor(2^(31 + l) / bs) + 1 < 2^32 exceeds 2^(31 + l) / bs by
-// at most 1, so key m / 2^(31 + l) passes key / bs by less than 1 / bs.
-void set_divisor(TreeParams& p) {
+// Multiplier and shift for exact quotients by d of numbers below 2^31 (0: a shift
+// alone). With l = ceil(log2 d), m = floor(2^(31 + l) / d) + 1 < 2^32 exceeds
+// 2^(31 + l) / d by at most 1, so x m / 2^(31 + l) passes x / d by less than 1 / d.
+void divisor(int d, uint32_t* mul, int* shift) {
   int l = 0;
-  while ((1LL << l) < p.bs) ++l;
-  const bool power = (1LL << l) == p.bs;
-  p.bs_mul = power ? 0u : static_cast<uint32_t>((1ull << (31 + l)) / p.bs + 1);
-  p.bs_shift = power ? l : l - 1;
+  while ((1LL << l) < d) ++l;
+  const bool power = (1LL << l) == d;
+  *mul = power ? 0u : static_cast<uint32_t>((1ull << (31 + l)) / d + 1);
+  *shift = power ? l : l - 1;
 }
 
 int run(TreeParams& p, int T, int H, int D, float scale, int dtype, int fmt, void* workspace,
@@ -182,7 +193,8 @@ int run(TreeParams& p, int T, int H, int D, float scale, int dtype, int fmt, voi
   if (need > 0 && (workspace == nullptr || workspace_bytes < need ||
                    (reinterpret_cast<uintptr_t>(workspace) & 15u) != 0))
     return LK_ERR_WORKSPACE;
-  set_divisor(p);
+  divisor(p.bs, &p.bs_mul, &p.bs_shift);
+  divisor(p.G, &p.g_mul, &p.g_shift);
   p.scale_log2 = scale * 1.4426950408889634f;
   p.cluster = r.cluster;
   p.chunk = r.chunk;

@@ -9,7 +9,7 @@
 // s = 1 for 16-bit caches. GQA: the n * G query rows of a KV head share its keys.
 //
 // The keys are read once for up to 32 query rows and 4 H D operations a key, so
-// HBM bounds it while n * G is small. Layout:
+// HBM bounds it while n * G is small (with many rows paged_tree_tc.cuh runs). Layout:
 //  * CTA = (KV head, 8 NT query rows, split of the context, sequence), four
 //    warps. Each warp streams its own stages of kTok keys (warp w takes stages
 //    w, w + 4, ...) with 16-byte cp.async through a private ring: no barrier
@@ -131,10 +131,7 @@ paged_tree_kernel(const TreeParams p) {
   u /= p.H_kv;
   const int b = u % p.B;
   if (p.cluster == 1) sp = u / p.B;
-  auto quotient = [&](int key) {
-    return static_cast<int>(p.bs_mul ? __umulhi(key, p.bs_mul) >> p.bs_shift
-                                     : static_cast<uint32_t>(key) >> p.bs_shift);
-  };
+  auto quotient = [&](int key) { return tree_quotient(p, key); };
   const int32_t* bt = p.block_tables + static_cast<int64_t>(b) * p.bt_stride;
   // Where the split's start does not depend on the context's length, the first
   // stage's block is read beside that length, not after it.
@@ -224,8 +221,9 @@ paged_tree_kernel(const TreeParams p) {
   // ------------------------------------------------------ queries to smem ---
   for (int j = warp; j < COLS; j += kWarps) {
     const int r = cg * COLS + j;
-    const int token = r < rows ? r / p.G : -1;
-    const int head = kvh * p.G + r % p.G;
+    const int tok = tree_token(p, r);
+    const int token = r < rows ? tok : -1;
+    const int head = kvh * p.G + r - tok * p.G;
     const T* src = static_cast<const T*>(p.q) +
                    static_cast<int64_t>(row0 + max(token, 0)) * p.q_stride +
                    static_cast<int64_t>(head) * D;
@@ -666,8 +664,7 @@ paged_tree_kernel(const TreeParams p) {
 
   // ------------------------------------------------------ join the cluster ---
   // CTA r of the cluster joins columns r, r + n, ..., in split order.
-  namespace cg_ = cooperative_groups;
-  cg_::cluster_group cluster = cg_::this_cluster();
+  cooperative_groups::cluster_group cluster = cooperative_groups::this_cluster();
   cluster.sync();
   const int n_cta = min(p.cluster, max(1, (ctx + chunk - 1) / max(chunk, 1)));  // that held keys
   for (int j = sp + warp * p.cluster; j < COLS; j += kWarps * p.cluster) {

@@ -1,6 +1,6 @@
-// Parameters and launchers of the drafted-tree / 8-bit-cache attention
-// kernel (paged_tree.cuh), one launcher per cache format so that the
-// instantiations compile in separate files.
+// Parameters and launchers of the drafted-tree / 8-bit-cache attention kernels
+// (paged_tree.cuh on mma.sync, paged_tree_tc.cuh on tcgen05), one launcher per
+// cache format so that the instantiations compile in separate files.
 #pragma once
 
 #include "lk_host.h"
@@ -28,6 +28,8 @@ struct TreeParams {
   int B, H_kv, G, bs, max_blocks;
   uint32_t bs_mul;              // key / bs: key >> bs_shift if 0, else umulhi(key, bs_mul) >> bs_shift
   int bs_shift;
+  uint32_t g_mul;               // row / G in the same way
+  int g_shift;
   int64_t num_blocks;
   int max_q;                    // most query tokens of a sequence
   float scale_log2;             // scale * log2(e)
@@ -38,7 +40,20 @@ struct TreeParams {
   float* part_o;                // [T * H][nsplit][D]
 };
 
-// NT (1, 2, 4): groups of eight query rows a CTA takes.
+#ifdef __CUDACC__
+// key / p.bs, key < 2^31.
+__device__ __forceinline__ int tree_quotient(const TreeParams& p, int key) {
+  return static_cast<int>(p.bs_mul ? __umulhi(key, p.bs_mul) >> p.bs_shift
+                                   : static_cast<uint32_t>(key) >> p.bs_shift);
+}
+// Query token of a KV head's query row, row / G.
+__device__ __forceinline__ int tree_token(const TreeParams& p, int row) {
+  return static_cast<int>(p.g_mul ? __umulhi(row, p.g_mul) >> p.g_shift
+                                  : static_cast<uint32_t>(row) >> p.g_shift);
+}
+#endif
+
+// NT (1, 2, 4): groups of eight query rows a CTA takes; 0: the tcgen05 kernel.
 int tree_launch_16(const TreeParams& p, int dtype, int D, int NT, unsigned grid, cudaStream_t s);
 int tree_launch_i8(const TreeParams& p, int dtype, int D, int NT, unsigned grid, cudaStream_t s);
 int tree_launch_e4m3(const TreeParams& p, int dtype, int D, int NT, unsigned grid, cudaStream_t s);

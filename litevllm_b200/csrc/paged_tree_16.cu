@@ -1,10 +1,12 @@
-// The drafted-tree attention kernel over LK_KV_16BIT caches.
+// The drafted-tree attention kernels over LK_KV_16BIT caches.
 #include "paged_tree.cuh"
+#include "paged_tree_tc.cuh"
 
 namespace lk {
 
 int tree_launch_16(const TreeParams& p, int dtype, int D, int NT, unsigned grid, cudaStream_t s) {
-  return tree::by_type<LK_KV_16BIT>(p, dtype, D, NT, grid, s);
+  return NT == 0 ? treetc::by_type<LK_KV_16BIT>(p, dtype, D, grid, s)
+                 : tree::by_type<LK_KV_16BIT>(p, dtype, D, NT, grid, s);
 }
 
 }  // namespace lk

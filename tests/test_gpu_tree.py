@@ -63,6 +63,12 @@ SHAPES = [  # (H, H_kv, D, bs, ctx, counts)
     (16, 2, 64, 16, [600, 128, 45], [2, 1, 2]),                      # 16 rows
     (12, 1, 128, 32, [515, 80], [64, 40]),                           # G = 12
     (4, 2, 64, 16, [400, 129], [130, 70]),                           # masks of three words
+    # enough work for the tcgen05 kernel: 16-row groups to several tiles of 128 rows
+    (32, 8, 128, 16, [2100, 700, 64, 33], [40, 64, 64, 1]),
+    (8, 2, 64, 32, [1500, 900], [100, 130]),
+    (20, 4, 128, 48, [900, 1300, 0], [60, 17, 0]),                   # G = 5
+    (24, 1, 64, 16, [4097], [24]),                                   # G = 24, many splits
+    (32, 8, 128, 16, [2049] * 3, [8] * 3),                           # one key past a split
 ]
 
 
@@ -94,15 +100,19 @@ def test_rows_that_see_nothing_are_nan(cuda, kind):
 @pytest.mark.parametrize("kind", [BF16, F16, INT8, E4M3])
 @pytest.mark.parametrize("where", ["k", "v"])
 @pytest.mark.parametrize("value", [float("nan"), float("inf"), -float("inf")])
-def test_special_values_in_hidden_drafts_do_not_leak(cuda, kind, where, value):
+@pytest.mark.parametrize("shape", [(8, 2, 128, 16, [50, 37], [9, 20]),
+                                   (32, 8, 128, 16, [600, 337], [40, 64]),
+                                   (32, 8, 64, 32, [651, 300], [40, 64])], ids=range(3))
+def test_special_values_in_hidden_drafts_do_not_leak(cuda, kind, where, value, shape):
     """A drafted token with a NaN or an infinity changes the rows that see it and
     no other."""
     dtype = kind if kind in (BF16, F16) else BF16
-    c = case(kind, dtype, 8, 2, 128, 16, [50, 37], [9, 20], seed=8)
+    c = case(kind, dtype, *shape, seed=8)
     bad = 2  # of both sequences, seen by its descendants only
     for b, (n, ctx) in enumerate(zip(c["counts"], c["ctx"])):
         key = ctx - n + bad
-        blk, off = c["tables"][b, key // 16], key % 16
+        bs = c["kd"].shape[1]
+        blk, off = c["tables"][b, key // bs], key % bs
         if c["ks"] is None:
             c[where + "d"][blk, off, :, 5:7] = value
         else:  # the 8-bit store keeps such a row as zeros with scale NaN
@@ -182,16 +192,53 @@ def test_decode_and_chain_of_one_agree(cuda):
         check(c, got)
 
 
+@pytest.mark.parametrize("kind", [BF16, F16, INT8, E4M3])
+@pytest.mark.parametrize("D", [64, 128])
+def test_stale_rows_behind_a_context_are_not_used(cuda, kind, D):
+    """What other sequences left behind a context in its last block may be NaN; more
+    than one split, and a last chunk with few keys."""
+    dtype = kind if kind in (BF16, F16) else BF16
+    c = case(kind, dtype, 32, 8, D, 32, [2055, 1000, 37], [8, 40, 33], seed=6)
+    for b, ctx in enumerate(c["ctx"]):
+        blk, off = c["tables"][b, ctx // 32], ctx % 32
+        for x in ("k", "v"):
+            if c["ks"] is None:
+                c[x + "d"][blk, off:] = float("nan")
+            else:
+                c[x + "d"].view(torch.uint8)[blk, off:] = 0x7F  # NaN in e4m3
+                c[x + "s"][blk, :, off:] = float("nan")
+    check(c, run(c, cuda))
+    q = c["q"][:3]
+    if c["ks"] is not None:
+        got = ops.paged_decode_q8(q.cuda(), on(cuda, c["kd"], c["ks"]), on(cuda, c["vd"], c["vs"]),
+                                  c["tables"].cuda(), torch.tensor(c["ctx"], dtype=torch.int32).cuda(),
+                                  c["scale"])
+        want, size = tree_attention.decode(q, c["kd"], c["ks"], c["vd"], c["vs"], c["tables"], c["ctx"], c["scale"])
+        assert_attention(got, want, size, q, row_bounds(c["kd"], c["ks"], c["vd"], c["vs"]), c["scale"],
+                         max(c["ctx"]), 2.0 ** -11)
+
+
+@pytest.mark.parametrize("kind", [BF16, INT8])
+@pytest.mark.parametrize("scale", [0.0, -0.3, 4.0])
+def test_any_scale(cuda, kind, scale):
+    for shape in ((8, 2, 64, 16, [90, 300], [6, 9]), (32, 8, 64, 16, [700, 300], [40, 64])):
+        c = case(kind, BF16, *shape, seed=2)
+        c["scale"] = scale
+        check(c, run(c, cuda))
+
+
 @pytest.mark.parametrize("kind", [BF16, E4M3])
-def test_streams_and_graphs_do_not_share_state(cuda, kind):
+@pytest.mark.parametrize("rows", ["few", "many"])
+def test_streams_and_graphs_do_not_share_state(cuda, kind, rows):
     """Two captured graphs of split calls replayed at once on two streams, and
     eager calls beside them, give each its own result."""
-    cs = [case(kind, BF16, 8, 2, 128, 16, [3000 + 50 * i, 900], [6, 3], seed=10 + i) for i in range(2)]
+    n = [6, 3] if rows == "few" else [64, 50]
+    cs = [case(kind, BF16, 8, 2, 128, 16, [3000 + 50 * i, 900], n, seed=10 + i) for i in range(2)]
     state, want, graphs, outs = [], [], [], []
     for c in cs:
         state.append((c["q"].cuda(), on(cuda, c["kd"], c["ks"]), on(cuda, c["vd"], c["vs"]),
                       c["tables"].cuda(), torch.tensor(c["ctx"], dtype=torch.int32).cuda(),
-                      c["cu"].cuda(), 6, c["scale"], c["mask"].cuda()))
+                      c["cu"].cuda(), max(n), c["scale"], c["mask"].cuda()))
     call = lambda s: ops.paged_tree_attention(*s[:8], tree_mask=s[8])  # noqa: E731
     want = [call(s) for s in state]
     for c, w in zip(cs, want):

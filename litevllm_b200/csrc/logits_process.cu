@@ -10,11 +10,15 @@
 // (litevllm/layers/sampler.py:190-201); the others have no counterpart there.
 //
 // Bytes bound it: B * V logits in, B * V out, the mask's bits and the
-// histories. CTA = (part of the vocabulary, row): it counts the row's history
-// tokens that fall into its part in shared memory (top bit: in the prompt, the
-// rest: occurrences in the output), so no [B, V] count tensor exists, while
-// its logits are already on their way to registers. A part that the mask
-// closes is not read, and in place only what changes is written.
+// histories. CTA = (part of the vocabulary, row). Its logits go from global memory
+// through registers and back with the mask applied, a dense pass that knows
+// nothing of tokens; a vector that the mask closes is not read, and in place only
+// closed tokens are written. Meanwhile the CTA counts the row's history tokens of
+// its part in shared memory (so no [B, V] count tensor exists) and lists them, and
+// after the dense pass computes those few tokens, and the biased ones, again from
+// their logits. Reading the counts for every vector instead took 40 us on
+// 128 x 151936 with 16 biases and histories of up to 1024 + 512 tokens (now 26,
+// a bare copy 11).
 // Rows whose addresses are not multiples of 16 bytes keep 16-byte accesses:
 // tokens are indexed from the aligned address in front of the row.
 #include "lk_common.cuh"
@@ -24,8 +28,29 @@ namespace {
 
 constexpr int kLThreads = 256;
 constexpr int kLVecs = 4;        // 16-byte vectors per thread
+constexpr int kLCtas = 5;        // CTAs per SM (4: 28.3 us, 5: 26.5, 6: 28.2 with spills)
 constexpr int kLMaxBias = 1024;  // bias entries per row
-constexpr uint32_t kInPrompt = 0x80000000u;
+constexpr int kLList = 2048;     // listed history tokens of a part; more: all counts are looked at
+
+// What is known of a token, in C bits: in the prompt (top bit), biased (the next),
+// occurrences in the output. 16 bits, two tokens a word, for outputs of up to 16383
+// tokens: half the shared memory.
+template <int C> struct Marks {
+  static constexpr uint32_t kInPrompt = 1u << (C - 1), kBiased = 1u << (C - 2),
+                            kCount = kBiased - 1u;
+  LK_DEVINL static uint32_t get(const uint32_t* s, int at) {
+    return C == 32 ? s[at] : (s[at >> 1] >> ((at & 1) * 16)) & 0xffffu;
+  }
+  // both return what was there before
+  LK_DEVINL static uint32_t set(uint32_t* s, int at, uint32_t bits) {
+    if (C == 32) return atomicOr(&s[at], bits);
+    return (atomicOr(&s[at >> 1], bits << ((at & 1) * 16)) >> ((at & 1) * 16)) & 0xffffu;
+  }
+  LK_DEVINL static uint32_t count(uint32_t* s, int at) {
+    if (C == 32) return atomicAdd(&s[at], 1u);
+    return (atomicAdd(&s[at >> 1], 1u << ((at & 1) * 16)) >> ((at & 1) * 16)) & 0xffffu;
+  }
+};
 
 struct LogitsParams {
   const void* logits;
@@ -55,12 +80,29 @@ struct LogitsParams {
 template <typename T> struct Raw;
 template <> struct Raw<float> {
   static constexpr int kVe = 4;
+  // v where bit i of `open` allows its tokens, -inf elsewhere
+  LK_DEVINL static uint4 masked(uint4 v, uint32_t open) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (!((open >> i) & 1u)) (&v.x)[i] = 0xff800000u;
+    return v;
+  }
   LK_DEVINL static float get(const uint4& v, int i) { return __uint_as_float((&v.x)[i]); }
   LK_DEVINL static void put(uint4& v, int i, float x) { (&v.x)[i] = __float_as_uint(x); }
   LK_DEVINL static float round(float x) { return x; }
 };
 template <typename T> struct Raw16 {
   static constexpr int kVe = 8;
+  LK_DEVINL static uint4 masked(uint4 v, uint32_t open) {
+    constexpr uint32_t inf = lk::Elem<T>::code == LK_DTYPE_BF16 ? 0xff80ff80u : 0xfc00fc00u;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t m = ((open >> (2 * i)) & 1u ? 0x0000ffffu : 0u) |
+                         ((open >> (2 * i)) & 2u ? 0xffff0000u : 0u);
+      (&v.x)[i] = ((&v.x)[i] & m) | (inf & ~m);
+    }
+    return v;
+  }
   LK_DEVINL static float get(const uint4& v, int i) {
     const uint16_t h = static_cast<uint16_t>((&v.x)[i >> 1] >> ((i & 1) * 16));
     return lk::Elem<T>::to_f(*reinterpret_cast<const T*>(&h));
@@ -82,22 +124,25 @@ struct RowTerms {
   float rep, pres, freq;
 };
 
-LK_DEVINL float process(float x, uint32_t seen, const RowTerms& r) {
-  if (seen == 0u) return x;
+template <int C> LK_DEVINL float process(float x, uint32_t seen, const RowTerms& r) {
+  if ((seen & ~Marks<C>::kBiased) == 0u) return x;
   x = x > 0.f ? __fdiv_rn(x, r.rep) : __fmul_rn(x, r.rep);
-  const uint32_t c = seen & ~kInPrompt;
+  const uint32_t c = seen & Marks<C>::kCount;
   const float p = c ? __fadd_rn(__fmul_rn(r.freq, static_cast<float>(c)), r.pres) : 0.f;
   return __fsub_rn(x, p);
 }
 
-template <typename T, bool VEC>
-__global__ void __launch_bounds__(kLThreads) logits_process_kernel(const LogitsParams p) {
+template <typename T, bool VEC, int C>
+__global__ void __launch_bounds__(kLThreads, kLCtas) logits_process_kernel(const LogitsParams p) {
   constexpr int VE = Raw<T>::kVe;
   constexpr int CH = kLThreads * kLVecs * VE;  // tokens per CTA
-  extern __shared__ uint32_t seen[];           // [CH], then the biases
-  float* bias_x = reinterpret_cast<float*>(seen + CH);        // [nbias] results
-  float* bias_v = bias_x + p.nbias;                            // [nbias]
-  int* bias_t = reinterpret_cast<int*>(bias_v + p.nbias);      // [nbias] token or -1
+  constexpr uint32_t kAll = (1u << VE) - 1u;
+  using Mk = Marks<C>;
+  extern __shared__ __align__(16) uint32_t seen[];            // [CH] marks, only with sparse terms
+  uint16_t* list = reinterpret_cast<uint16_t*>(seen + CH * C / 32);  // [kLList] seen tokens
+  float* bias_v = reinterpret_cast<float*>(list + kLList);    // [nbias]
+  int* bias_t = reinterpret_cast<int*>(bias_v + p.nbias);     // [nbias] token or -1
+  __shared__ int listed;
   const int b = blockIdx.y, tid = threadIdx.x;
   const T* in = static_cast<const T*>(p.logits) + b * p.ld;
   T* out = static_cast<T*>(p.out) + b * p.out_ld;
@@ -108,35 +153,56 @@ __global__ void __launch_bounds__(kLThreads) logits_process_kernel(const LogitsP
   const int a1 = min(a0 + CH, p.V + shift);
   if (a0 >= a1) return;
   const uint32_t* allowed = p.allowed ? p.allowed + b * p.allowed_ld : nullptr;
-  const int words = (p.V + 31) >> 5;
 
   RowTerms r;
   r.rep = p.repetition ? p.repetition[b] : 1.f;
   r.pres = p.presence ? p.presence[b] : 0.f;
   r.freq = p.frequency ? p.frequency[b] : 0.f;
-  const bool counts = r.pres != 0.f || r.freq != 0.f;
-  const bool past = counts || r.rep != 1.f;
-
-  // which tokens of each vector exist (bits 0..VE-1) and are allowed
+  const bool past = r.pres != 0.f || r.freq != 0.f || r.rep != 1.f;
+  const bool sparse = past || p.nbias > 0;
+  // ------------------------------------------------ dense: loads under way ---
+  // which tokens of each vector exist (live) and are allowed (open), a bit each
   uint32_t live[kLVecs], open[kLVecs];
   uint4 x[kLVecs];
+  const bool inner = VEC && a0 >= shift && a0 + CH - shift <= p.V;  // every vector whole
+  if (inner) {
+    const int v0 = a0 - shift + tid * VE;
 #pragma unroll
-  for (int k = 0; k < kLVecs; ++k) {
-    const int v = a0 + (k * kLThreads + tid) * VE - shift;
-    const int skip = max(-v, 0), left = min(max(p.V - v, 0), VE);
-    live[k] = left > skip ? ((1u << left) - 1u) & ~((1u << skip) - 1u) : 0u;
-    open[k] = live[k];
-    if (allowed && live[k]) {
-      const int at = max(v, 0) >> 5, sh = max(v, 0) & 31;
-      uint64_t w = __ldg(allowed + at);
-      if (sh + VE > 32 && at + 1 < words) w |= static_cast<uint64_t>(__ldg(allowed + at + 1)) << 32;
-      open[k] &= static_cast<uint32_t>(w >> sh) << skip;
+    for (int k = 0; k < kLVecs; ++k) {
+      live[k] = open[k] = kAll;
+      if (allowed) {
+        const int v = v0 + k * kLThreads * VE;
+        if (shift == 0) {  // a vector's bits are a byte or half of one
+          open[k] = (__ldg(reinterpret_cast<const uint8_t*>(allowed) + (v >> 3)) >> (v & 7)) & kAll;
+        } else {
+          const uint32_t lo = __ldg(allowed + (v >> 5));
+          const uint32_t hi = (v & 31) + VE > 32 ? __ldg(allowed + (v >> 5) + 1) : 0u;
+          open[k] = __funnelshift_r(lo, hi, v & 31) & kAll;
+        }
+      }
     }
-    x[k] = make_uint4(0u, 0u, 0u, 0u);
-    if (open[k]) {
-      if (VEC && live[k] == (1u << VE) - 1u) {
+#pragma unroll
+    for (int k = 0; k < kLVecs; ++k)
+      x[k] = open[k] ? *reinterpret_cast<const uint4*>(in + v0 + k * kLThreads * VE)
+                     : make_uint4(0u, 0u, 0u, 0u);
+  } else {
+    const int words = (p.V + 31) >> 5;
+#pragma unroll
+    for (int k = 0; k < kLVecs; ++k) {
+      const int v = a0 + (k * kLThreads + tid) * VE - shift;
+      const int skip = max(-v, 0), left = min(max(p.V - v, 0), VE);
+      live[k] = left > skip ? ((1u << left) - 1u) & ~((1u << skip) - 1u) : 0u;
+      open[k] = live[k];
+      if (allowed && live[k]) {
+        const int at = max(v, 0) >> 5, sh = max(v, 0) & 31;
+        const uint32_t lo = __ldg(allowed + at);
+        const uint32_t hi = sh + VE > 32 && at + 1 < words ? __ldg(allowed + at + 1) : 0u;
+        open[k] &= __funnelshift_r(lo, hi, sh) << skip;
+      }
+      x[k] = make_uint4(0u, 0u, 0u, 0u);
+      if (VEC && open[k] && live[k] == kAll) {
         x[k] = *reinterpret_cast<const uint4*>(in + v);
-      } else {
+      } else if (open[k]) {
 #pragma unroll
         for (int i = 0; i < VE; ++i)
           if ((live[k] >> i) & 1u) Raw<T>::put(x[k], i, lk::Elem<T>::to_f(in[v + i]));
@@ -144,29 +210,11 @@ __global__ void __launch_bounds__(kLThreads) logits_process_kernel(const LogitsP
     }
   }
 
-  if (past) {
-    for (int i = tid; i < CH; i += kLThreads) seen[i] = 0u;
-    __syncthreads();
-    auto scan = [&](const int64_t* ids, int n, bool prompt) {
-      for (int i = tid; i < n; i += kLThreads) {
-        const int64_t id = ids[i];
-        if (id >= p.V && p.status && blockIdx.x == 0) atomicOr(p.status, LK_STATUS_TOKEN_OOB);
-        const int64_t at = id + shift - a0;
-        if (id < 0 || id >= p.V || at < 0 || at >= CH) continue;
-        if (prompt) atomicOr(&seen[at], kInPrompt);
-        else atomicAdd(&seen[at], 1u);
-      }
-    };
-    if (p.prompt_ids && r.rep != 1.f)
-      scan(p.prompt_ids + b * p.prompt_ld, p.prompt_lens ? min(p.prompt_lens[b], p.prompt_max) : p.prompt_max, true);
-    if (p.output_ids)
-      scan(p.output_ids + b * p.output_ld, p.output_lens ? min(p.output_lens[b], p.output_max) : p.output_max, false);
-    __syncthreads();
-  }
-  auto seen_at = [&](int v) { return past ? seen[v + shift - a0] : 0u; };
-
-  // Biased tokens of this part: computed before anything is overwritten.
-  if (p.nbias > 0) {
+  // ------------------------------------- the part's history and its biases ---
+  if (sparse) {
+    for (int i = tid; i < CH * C / 128; i += kLThreads)
+      reinterpret_cast<uint4*>(seen)[i] = make_uint4(0u, 0u, 0u, 0u);
+    if (tid == 0) listed = 0;
     for (int j = tid; j < p.nbias; j += kLThreads) {
       const int64_t id = p.bias_ids[static_cast<int64_t>(b) * p.nbias + j];
       if (id >= p.V && p.status && blockIdx.x == 0) atomicOr(p.status, LK_STATUS_TOKEN_OOB);
@@ -174,44 +222,45 @@ __global__ void __launch_bounds__(kLThreads) logits_process_kernel(const LogitsP
       bias_v[j] = p.bias[static_cast<int64_t>(b) * p.nbias + j];
     }
     __syncthreads();
-    for (int j = tid; j < p.nbias; j += kLThreads) {
-      const int v = bias_t[j];
-      if (v < 0 || v + shift < a0 || v + shift >= a1) continue;
-      bool first = true;
-      for (int i = 0; i < j && first; ++i) first = bias_t[i] != v;
-      if (!first) continue;
-      float sum = 0.f;
-      for (int i = j; i < p.nbias; ++i)
-        if (bias_t[i] == v) sum = __fadd_rn(sum, bias_v[i]);
-      bias_x[j] = __fadd_rn(process(lk::Elem<T>::to_f(in[v]), seen_at(v), r), sum);
+    auto note = [&](int64_t id, bool prompt) {
+      if (id >= p.V && p.status && blockIdx.x == 0) atomicOr(p.status, LK_STATUS_TOKEN_OOB);
+      const int64_t at = id + shift - a0;
+      if (id < 0 || id >= p.V || at < 0 || at >= CH) return;
+      const uint32_t was = prompt ? Mk::set(seen, static_cast<int>(at), Mk::kInPrompt)
+                                  : Mk::count(seen, static_cast<int>(at));
+      if ((was & ~Mk::kBiased) == 0u) {  // its first occurrence
+        const int n = atomicAdd(&listed, 1);
+        if (n < kLList) list[n] = static_cast<uint16_t>(at);
+      }
+    };
+    if (past) {
+      if (p.prompt_ids && r.rep != 1.f) {
+        const int64_t* ids = p.prompt_ids + b * p.prompt_ld;
+        const int n = p.prompt_lens ? min(p.prompt_lens[b], p.prompt_max) : p.prompt_max;
+#pragma unroll 4
+        for (int i = tid; i < n; i += kLThreads) note(__ldg(ids + i), true);
+      }
+      if (p.output_ids) {
+        const int64_t* ids = p.output_ids + b * p.output_ld;
+        const int n = p.output_lens ? min(p.output_lens[b], p.output_max) : p.output_max;
+#pragma unroll 4
+        for (int i = tid; i < n; i += kLThreads) note(__ldg(ids + i), false);
+      }
     }
-    __syncthreads();
+    for (int j = tid; j < p.nbias; j += kLThreads) {
+      const int at = bias_t[j] + shift - a0;
+      if (bias_t[j] >= 0 && at >= 0 && at < CH) Mk::set(seen, at, Mk::kBiased);
+    }
   }
 
+  // ---------------------------------------------------------- dense: stores ---
 #pragma unroll
   for (int k = 0; k < kLVecs; ++k) {
     if (!live[k]) continue;
-    const int at = (k * kLThreads + tid) * VE;
-    const int v = a0 + at - shift;
-    bool change = open[k] != live[k];
-    if (past && open[k]) {
-#pragma unroll
-      for (int i = 0; i < VE; i += 4) {
-        const uint4 s = *reinterpret_cast<const uint4*>(seen + at + i);
-        if ((s.x | s.y | s.z | s.w) == 0u) continue;
-        change = true;
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if ((&s.x)[j]) Raw<T>::put(x[k], i + j, process(Raw<T>::get(x[k], i + j), (&s.x)[j], r));
-      }
-    }
-    if (open[k] != live[k]) {
-#pragma unroll
-      for (int i = 0; i < VE; ++i)
-        if (!((open[k] >> i) & 1u)) Raw<T>::put(x[k], i, -INFINITY);
-    }
-    if (in_place && !change) continue;
-    if (VEC && live[k] == (1u << VE) - 1u) {
+    const int v = a0 + (k * kLThreads + tid) * VE - shift;
+    if (open[k] != live[k]) x[k] = Raw<T>::masked(x[k], open[k]);
+    else if (in_place) continue;
+    if (VEC && (inner || live[k] == kAll)) {
       *reinterpret_cast<uint4*>(out + v) = x[k];
     } else {
 #pragma unroll
@@ -219,18 +268,33 @@ __global__ void __launch_bounds__(kLThreads) logits_process_kernel(const LogitsP
         if ((live[k] >> i) & 1u) out[v + i] = Raw<T>::round(Raw<T>::get(x[k], i));
     }
   }
+  if (!sparse) return;
 
-  if (p.nbias > 0) {
-    __syncthreads();  // after the vectors that hold the same tokens
-    for (int j = tid; j < p.nbias; j += kLThreads) {
-      const int v = bias_t[j];
-      if (v < 0 || v + shift < a0 || v + shift >= a1) continue;
-      bool first = true;
-      for (int i = 0; i < j && first; ++i) first = bias_t[i] != v;
-      if (!first) continue;
-      const bool ok = !allowed || ((allowed[v >> 5] >> (v & 31)) & 1u);
-      out[v] = Raw<T>::round(ok ? bias_x[j] : -INFINITY);
-    }
+  // ---------------------------------- sparse: after the vectors around them ---
+  __syncthreads();
+  auto is_open = [&](int v) { return !allowed || ((allowed[v >> 5] >> (v & 31)) & 1u); };
+  auto one = [&](int at) {  // a history token without a bias
+    const uint32_t s = Mk::get(seen, at);
+    const int v = at + a0 - shift;
+    if (s == 0u || (s & Mk::kBiased) || !is_open(v)) return;
+    out[v] = Raw<T>::round(process<C>(lk::Elem<T>::to_f(in[v]), s, r));
+  };
+  if (listed <= kLList) {
+    for (int i = tid; i < listed; i += kLThreads) one(list[i]);
+  } else {
+    for (int i = tid; i < a1 - a0; i += kLThreads) one(i);
+  }
+  for (int j = tid; j < p.nbias; j += kLThreads) {
+    const int v = bias_t[j];
+    const int at = v + shift - a0;
+    if (v < 0 || at < 0 || at >= CH || !is_open(v)) continue;
+    bool first = true;  // the first entry of a token adds up all of them
+    for (int i = 0; i < j && first; ++i) first = bias_t[i] != v;
+    if (!first) continue;
+    float sum = 0.f;
+    for (int i = j; i < p.nbias; ++i)
+      if (bias_t[i] == v) sum = __fadd_rn(sum, bias_v[i]);
+    out[v] = Raw<T>::round(__fadd_rn(process<C>(lk::Elem<T>::to_f(in[v]), Mk::get(seen, at), r), sum));
   }
 }
 
@@ -238,7 +302,9 @@ template <typename T>
 int launch_logits(const LogitsParams& p, int B, cudaStream_t s) {
   constexpr int CH = kLThreads * kLVecs * Raw<T>::kVe;
   const int parts = (p.V + 15 + CH - 1) / CH;  // room for the shift
-  const size_t smem = CH * 4 + static_cast<size_t>(p.nbias) * 12;
+  const bool sparse = p.repetition || p.presence || p.frequency || p.nbias > 0;
+  const bool small = !p.output_ids || p.output_max <= static_cast<int>(Marks<16>::kCount);
+  const size_t smem = sparse ? CH * (small ? 2 : 4) + kLList * 2 + static_cast<size_t>(p.nbias) * 8 : 0;
   const bool vec =
       ((reinterpret_cast<uintptr_t>(p.logits) ^ reinterpret_cast<uintptr_t>(p.out)) & 15u) == 0 &&
       (((p.ld - p.out_ld) * static_cast<int64_t>(sizeof(T))) & 15) == 0;
@@ -250,7 +316,9 @@ int launch_logits(const LogitsParams& p, int B, cudaStream_t s) {
     kernel<<<dim3(parts, B), kLThreads, smem, s>>>(p);
     return lk::check_launch();
   };
-  return vec ? go(logits_process_kernel<T, true>) : go(logits_process_kernel<T, false>);
+  if (small)
+    return vec ? go(logits_process_kernel<T, true, 16>) : go(logits_process_kernel<T, false, 16>);
+  return vec ? go(logits_process_kernel<T, true, 32>) : go(logits_process_kernel<T, false, 32>);
 }
 
 }  // namespace

@@ -8,11 +8,13 @@ include/litekern.h one for one.
 from __future__ import annotations
 
 import ctypes
+import importlib.util
 import threading
 from ctypes import c_float, c_int32, c_int64, c_size_t, c_uint64, c_void_p
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "liblitekern.so"
+SPEC_PATH = LIB_PATH.with_name("_spec.so")
 
 LK_OK = 0
 LK_DTYPE_F32, LK_DTYPE_F16, LK_DTYPE_BF16 = 0, 1, 2
@@ -172,6 +174,22 @@ def lib() -> ctypes.CDLL:
                 fn.argtypes = args
             _lib = handle
     return _lib
+
+
+def spec_module():
+    """Load the native binding _spec.so (csrc/spec_binding.cpp). Raises if absent."""
+    lib()  # the binding calls into it
+    if not SPEC_PATH.exists():
+        raise LiteKernError(
+            f"{SPEC_PATH} is missing: build it with `python -m litevllm_b200.build`; "
+            "there is no fallback implementation"
+        )
+    import torch  # noqa: F401  (its libraries, which the binding links to)
+
+    spec = importlib.util.spec_from_file_location("litevllm_b200._spec", SPEC_PATH)
+    module = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(module)
+    return module
 
 
 def check(code: int) -> None:

@@ -4,7 +4,8 @@
     python -m litevllm_b200.build --force  # rebuild everything
 
 Objects go to litevllm_b200/_build/, the shared library to
-litevllm_b200/liblitekern.so, next to the ctypes loader that opens it.
+litevllm_b200/liblitekern.so, next to the ctypes loader that opens it, and the
+CPython binding of csrc/spec_binding.cpp to litevllm_b200/_spec.so.
 """
 
 from __future__ import annotations
@@ -14,6 +15,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
@@ -21,6 +23,7 @@ PKG = Path(__file__).resolve().parent
 CSRC = PKG / "csrc"
 BUILD = PKG / "_build"
 LIB = PKG / "liblitekern.so"
+SPEC = PKG / "_spec.so"
 INCLUDE = PKG.parent / "include"
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -78,7 +81,35 @@ def build(force: bool = False, verbose: bool = False) -> Path:
         if res.returncode != 0:
             raise RuntimeError(f"nvcc link failed:\n{res.stdout}\n{res.stderr}")
         os.replace(tmp, LIB)
+    build_spec(force, verbose)
     return LIB
+
+
+def build_spec(force: bool = False, verbose: bool = False) -> Path:
+    """The binding, with g++ against the installed torch; liblitekern.so comes first."""
+    import torch
+
+    src = CSRC / "spec_binding.cpp"
+    newest = max(p.stat().st_mtime for p in [src, *INCLUDE.glob("*.h")])
+    if not force and SPEC.exists() and SPEC.stat().st_mtime >= newest:
+        return SPEC
+    troot = Path(torch.__file__).resolve().parent
+    cuda = Path(nvcc()).resolve().parent.parent
+    tmp = SPEC.with_suffix(".so.tmp")
+    cmd = [
+        os.environ.get("CXX", "g++"), "-std=c++17", "-O2", "-fPIC", "-shared", f"-I{INCLUDE}",
+        f"-I{troot}/include", f"-I{troot}/include/torch/csrc/api/include", f"-I{cuda}/include",
+        f"-I{sysconfig.get_paths()['include']}", str(src), "-o", str(tmp), f"-L{PKG}",
+        "-l:liblitekern.so", f"-L{troot}/lib", "-ltorch_python", "-ltorch_cpu", "-lc10_cuda", "-lc10",
+        "-Wl,-rpath,$ORIGIN",
+    ]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"g++ failed on {src.name}:\n{res.stdout}\n{res.stderr}")
+    os.replace(tmp, SPEC)
+    return SPEC
 
 
 def main(argv: list[str] | None = None) -> int:

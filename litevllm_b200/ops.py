@@ -15,7 +15,7 @@ from typing import NamedTuple, Optional, Union
 import torch
 
 from ._lib import (LK_DTYPE_BF16, LK_DTYPE_F16, LK_DTYPE_F32, LK_KV_16BIT, LK_KV_E4M3, LK_KV_INT8,
-                   check, lib)
+                   LiteKernError, check, lib, spec_module)
 
 _DTYPES = {torch.float32: LK_DTYPE_F32, torch.float16: LK_DTYPE_F16, torch.bfloat16: LK_DTYPE_BF16}
 
@@ -143,6 +143,21 @@ class QuantizedCache(NamedTuple):
     scale: torch.Tensor
 
 
+_SPEC = None
+
+
+def _spec():
+    """The native binding of the functions over 8-bit caches and drafted trees and
+    of process_logits: it checks, allocates and calls as the functions below do in
+    Python, in a quarter of the time, which bounds their small calls."""
+    global _SPEC
+    if _SPEC is None:
+        module = spec_module()
+        module.init(QuantizedCache, LiteKernError)
+        _SPEC = module
+    return _SPEC
+
+
 def new_quantized_cache(num_blocks: int, block_size: int, num_kv_heads: int, head_dim: int,
                         dtype: torch.dtype = torch.int8, device="cuda") -> QuantizedCache:
     """A zeroed 8-bit key or value cache (dtype torch.int8 or torch.float8_e4m3fn)."""
@@ -151,31 +166,6 @@ def new_quantized_cache(num_blocks: int, block_size: int, num_kv_heads: int, hea
     return QuantizedCache(
         torch.zeros((num_blocks, block_size, num_kv_heads, head_dim), dtype=dtype, device=device),
         torch.zeros((num_blocks, num_kv_heads, block_size), dtype=torch.float32, device=device))
-
-
-def _check_q8(key_cache: QuantizedCache, value_cache: QuantizedCache) -> int:
-    """Checks a pair of 8-bit caches; the LK_KV_* code."""
-    if not isinstance(key_cache, QuantizedCache) or not isinstance(value_cache, QuantizedCache):
-        raise TypeError("key_cache and value_cache must both be QuantizedCache")
-    kd, ks = key_cache
-    vd, vs = value_cache
-    if kd.dtype not in _KV_FORMATS or vd.dtype != kd.dtype:
-        raise TypeError("8-bit caches are both torch.int8 or both torch.float8_e4m3fn")
-    if ks.dtype != torch.float32 or vs.dtype != torch.float32:
-        raise TypeError("scales must be fp32")
-    if kd.dim() != 4 or vd.shape != kd.shape:
-        raise ValueError("cache data must be [num_blocks, block_size, H_kv, D] of equal shapes")
-    nb, bs, H_kv, _ = kd.shape
-    if ks.shape != (nb, H_kv, bs) or vs.shape != ks.shape:
-        raise ValueError("scales must be [num_blocks, H_kv, block_size]")
-    if not (kd.is_contiguous() and vd.is_contiguous() and ks.is_contiguous() and vs.is_contiguous()):
-        raise ValueError("caches and scales must be contiguous")
-    return _KV_FORMATS[kd.dtype]
-
-
-def _check_status(status: Optional[torch.Tensor]) -> None:
-    if status is not None and (status.dtype != torch.int32 or status.numel() < 1):
-        raise TypeError("status must be an int32 tensor")
 
 
 def store_kvcache_q8(
@@ -192,33 +182,7 @@ def store_kvcache_q8(
     key/value: fp16 / bf16 [T, H_kv, D], D 64 or 128; slot_mapping int64 [T],
     -1 skips a token.
     """
-    fmt = _check_q8(key_cache, value_cache)
-    dev = _cuda(key, value, *key_cache, *value_cache, slot_mapping, status)
-    if key.dim() != 3 or value.shape != key.shape:
-        raise ValueError("key/value must be [T, H_kv, D] with equal shapes")
-    T, H_kv, D = key.shape
-    nb, bs, Hc, Dc = key_cache.data.shape
-    if (Hc, Dc) != (H_kv, D):
-        raise ValueError("caches must be [num_blocks, block_size, H_kv, D]")
-    for t in (key, value):
-        if t.stride(2) != 1 or t.stride(1) != D:
-            raise ValueError("key/value must have unit d-stride and head stride D")
-    code = _dtype_code(key)
-    if value.dtype != key.dtype:
-        raise TypeError("key and value must share a dtype")
-    if slot_mapping.dtype != torch.int64 or slot_mapping.numel() != T:
-        raise TypeError("slot_mapping must be int64 [T]")
-    _check_status(status)
-    slot_mapping = slot_mapping.contiguous()
-    with _on(dev):
-        check(
-            lib().lk_store_kv_q8(
-                key.data_ptr(), value.data_ptr(), key_cache.data.data_ptr(),
-                key_cache.scale.data_ptr(), value_cache.data.data_ptr(),
-                value_cache.scale.data_ptr(), slot_mapping.data_ptr(), T, H_kv, D, key.stride(0),
-                value.stride(0), nb, bs, code, fmt, _ptr(status), _stream(dev),
-            )
-        )
+    _spec().store(key, value, key_cache, value_cache, slot_mapping, status)
 
 
 def load_kvcache_q8(
@@ -237,67 +201,8 @@ def load_kvcache_q8(
     (fp32, fp16 or bf16). Row cu_rows[b] + p is position p of sequence b;
     a sequence's rows past its context are zero, rows that belong to no sequence
     are left as they were. cu_rows int32 [B + 1]."""
-    fmt = _check_q8(key_cache, value_cache)
-    dev = _cuda(*key_cache, *value_cache, block_tables, context_lens, cu_rows, key_out, value_out,
-                status)
-    nb, bs, H_kv, D = key_cache.data.shape
-    if block_tables.dtype != torch.int32 or block_tables.dim() != 2:
-        raise TypeError("block_tables must be int32 [B, max_blocks]")
-    B, max_blocks = block_tables.shape
-    if max_blocks > 0 and block_tables.stride(1) != 1:
-        block_tables = block_tables.contiguous()
-    if context_lens.dtype != torch.int32 or context_lens.numel() != B:
-        raise TypeError("context_lens must be int32 [B]")
-    if cu_rows.dtype != torch.int32 or cu_rows.numel() != B + 1:
-        raise TypeError("cu_rows must be int32 [B + 1]")
-    _check_status(status)
-    context_lens, cu_rows = context_lens.contiguous(), cu_rows.contiguous()
-    num_rows = int(num_rows)
-    if num_rows < 0:
-        raise ValueError("num_rows must not be negative")
-    outs = []
-    for out in (key_out, value_out):
-        if out is None:
-            out = torch.empty((num_rows, H_kv, D), dtype=dtype, device=dev)
-        elif out.shape != (num_rows, H_kv, D) or out.dtype != dtype or not out.is_contiguous():
-            raise ValueError("key_out/value_out must be contiguous [num_rows, H_kv, D] of dtype")
-        outs.append(out)
-    code = _dtype_code(outs[0], (torch.float32, torch.float16, torch.bfloat16))
-    with _on(dev):
-        check(
-            lib().lk_load_kv_q8(
-                outs[0].data_ptr(), outs[1].data_ptr(), key_cache.data.data_ptr(),
-                key_cache.scale.data_ptr(), value_cache.data.data_ptr(),
-                value_cache.scale.data_ptr(), block_tables.data_ptr(), block_tables.stride(0),
-                context_lens.data_ptr(), cu_rows.data_ptr(), B, num_rows, H_kv, D, nb, bs,
-                max_blocks, code, fmt, _ptr(status), _stream(dev),
-            )
-        )
-    return tuple(outs)
-
-
-def _tree_workspace(dev, workspace, T, B, max_q, H, H_kv, D, bs, max_blocks, fmt):
-    """(pointer, bytes, tensor to keep alive). Without a caller's workspace the
-    partials of split contexts live in a buffer of this call's own, from torch's
-    allocator: calls on other streams and captured graphs never share it."""
-    key = (dev.index, T, B, max_q, H, H_kv, D, bs, max_blocks, fmt)
-    need = _TREE_WS.get(key)
-    if need is None:
-        if len(_TREE_WS) > 65536:  # token counts vary from step to step
-            _TREE_WS.clear()
-        need = _TREE_WS[key] = int(lib().lk_paged_tree_workspace_bytes(
-            T, B, max_q, H, H_kv, D, bs, max_blocks, fmt))
-    if workspace is None:
-        if need == 0:
-            return None, 0, None
-        workspace = torch.empty(need, dtype=torch.uint8, device=dev)
-    nbytes = workspace.numel() * workspace.element_size()
-    if nbytes < need:
-        raise ValueError(f"workspace too small: need {need} bytes")
-    return workspace.data_ptr(), nbytes, workspace
-
-
-_TREE_WS: dict = {}  # shape -> lk_paged_tree_workspace_bytes, asked once per shape
+    return _spec().load(key_cache, value_cache, block_tables, context_lens, cu_rows, num_rows, dtype,
+                        key_out, value_out, status)
 
 
 def tree_workspace_bytes(num_tokens: int, num_seqs: int, max_q_len: int, H: int, H_kv: int,
@@ -323,10 +228,8 @@ def paged_decode_q8(
 ) -> torch.Tensor:
     """paged_decode over 8-bit caches: query fp16 / bf16 [B, H, D] -> [B, H, D],
     D 64 or 128, any block size and G = H / H_kv. A context of 0 gives NaN rows."""
-    fmt = _check_q8(key_cache, value_cache)
-    dev = _cuda(query, *key_cache, *value_cache, block_tables, context_lens, out, workspace, status)
-    return _tree(dev, query, key_cache.data, key_cache.scale, value_cache.data, value_cache.scale,
-                 fmt, block_tables, context_lens, None, None, 1, scale, out, workspace, status)
+    return _spec().tree(query, key_cache, value_cache, block_tables, context_lens, None, None, scale,
+                        None, out, workspace, status)
 
 
 def paged_tree_attention(
@@ -353,83 +256,8 @@ def paged_tree_attention(
     mask the tokens are a chain (d <= i). A token that sees nothing is NaN.
     Caches: 16-bit tensors of the query's dtype or QuantizedCache pairs.
     """
-    if isinstance(key_cache, QuantizedCache) or isinstance(value_cache, QuantizedCache):
-        fmt = _check_q8(key_cache, value_cache)
-        (kd, ks), (vd, vs) = key_cache, value_cache
-    else:
-        fmt, kd, ks, vd, vs = LK_KV_16BIT, key_cache, None, value_cache, None
-    dev = _cuda(query, kd, ks, vd, vs, block_tables, context_lens, cu_seqlens_q, tree_mask, out,
-                workspace, status)
-    if fmt == LK_KV_16BIT:
-        if kd.dim() != 4 or vd.shape != kd.shape:
-            raise ValueError("cache shape mismatch")
-        if kd.dtype != query.dtype or vd.dtype != query.dtype:
-            raise TypeError("query dtype must match the cache dtype")
-        if not (kd.is_contiguous() and vd.is_contiguous()):
-            raise ValueError("caches must be contiguous")
-    if cu_seqlens_q.dtype != torch.int32 or cu_seqlens_q.numel() != block_tables.shape[0] + 1:
-        raise TypeError("cu_seqlens_q must be int32 [B + 1]")
-    max_q_len = int(max_q_len)
-    if max_q_len < 0:
-        raise ValueError("max_q_len must not be negative")
-    if tree_mask is not None:
-        if tree_mask.dtype != torch.int64 or tree_mask.dim() != 2 or tree_mask.shape[0] != query.shape[0]:
-            raise TypeError("tree_mask must be int64 [T, words]")
-        if tree_mask.shape[1] * 64 < max_q_len:
-            raise ValueError("tree_mask must have a bit for each of max_q_len tokens")
-        if tree_mask.stride(1) != 1:
-            tree_mask = tree_mask.contiguous()
-    return _tree(dev, query, kd, ks, vd, vs, fmt, block_tables, context_lens,
-                 cu_seqlens_q.contiguous(), tree_mask, max_q_len, scale, out, workspace, status)
-
-
-def _tree(dev, query, kd, ks, vd, vs, fmt, block_tables, context_lens, cu, mask, max_q, scale, out,
-          workspace, status):
-    if query.dim() != 3:
-        raise ValueError("query must be [T, H, D]")
-    T, H, D = query.shape
-    nb, bs, H_kv, Dk = kd.shape
-    if Dk != D:
-        raise ValueError("cache shape mismatch")
-    if query.stride(2) != 1 or query.stride(1) != D:
-        raise ValueError("query must have unit d-stride and head stride D")
-    if block_tables.dtype != torch.int32 or block_tables.dim() != 2:
-        raise TypeError("block_tables must be int32 [B, max_blocks]")
-    B, max_blocks = block_tables.shape
-    if cu is None and B != T:
-        raise ValueError("decode takes one query per row of block_tables")
-    if block_tables.stride(1) != 1 and max_blocks > 0:
-        block_tables = block_tables.contiguous()
-    if context_lens.dtype != torch.int32 or context_lens.numel() != B:
-        raise TypeError("context_lens must be int32 [B]")
-    context_lens = context_lens.contiguous()
-    code = _dtype_code(query)
-    _check_status(status)
-    if out is None:
-        out = torch.empty((T, H, D), dtype=query.dtype, device=dev)
-    elif out.shape != (T, H, D) or out.dtype != query.dtype or out.stride(2) != 1 or out.stride(1) != D:
-        raise ValueError("bad out tensor")
-    if T == 0 or B == 0 or max_q == 0:
-        return out
-    with _on(dev):
-        ws, ws_bytes, keep = _tree_workspace(dev, workspace, T, B, max_q, H, H_kv, D, bs,
-                                             max_blocks, fmt)
-        args = (B, H, H_kv, D, bs, max_blocks, float(scale), code, fmt, ws, ws_bytes, _ptr(status),
-                _stream(dev))
-        head = (out.data_ptr(), out.stride(0), query.data_ptr(), query.stride(0), kd.data_ptr(),
-                _ptr(ks), vd.data_ptr(), _ptr(vs), nb, block_tables.data_ptr(),
-                block_tables.stride(0))
-        if cu is None:
-            check(lib().lk_paged_decode_q8(*head, context_lens.data_ptr(), *args))
-        else:
-            check(
-                lib().lk_paged_tree_attention(
-                    *head, cu.data_ptr(), context_lens.data_ptr(), _ptr(mask),
-                    0 if mask is None else mask.stride(0), 0 if mask is None else mask.shape[1], T,
-                    B, max_q, *args[1:],
-                )
-            )
-    return out
+    return _spec().tree(query, key_cache, value_cache, block_tables, context_lens, cu_seqlens_q,
+                        max_q_len, scale, tree_mask, out, workspace, status)
 
 
 def tree_mask_from_parents(parents, device=None) -> torch.Tensor:
@@ -963,73 +791,8 @@ def process_logits(
     if logits.dim() == 1:
         logits = logits.unsqueeze(0)
         out = out.unsqueeze(0) if out is not None and out.dim() == 1 else out
-    dev = _cuda(logits, prompt_ids, prompt_lens, output_ids, output_lens, repetition, presence,
-                frequency, bias_ids, bias, allowed, out, status)
-    if logits.dim() != 2 or logits.shape[1] == 0:
-        raise ValueError("logits must be [B, V]")
-    B, V = logits.shape
-    code = _dtype_code(logits, (torch.float32, torch.float16, torch.bfloat16))
-    if logits.stride(1) != 1 or (B > 1 and logits.stride(0) < V):
-        if out is not None and out.data_ptr() == logits.data_ptr():
-            raise ValueError("in place, logits must have unit column stride and rows of their own")
-        logits = logits.contiguous()
-    ids_args = []
-    for name, ids, lens in (("prompt", prompt_ids, prompt_lens), ("output", output_ids, output_lens)):
-        if ids is None:
-            ids_args += [None, 0, None, 0]
-            continue
-        if ids.dtype != torch.int64 or ids.dim() != 2 or ids.shape[0] != B:
-            raise TypeError(f"{name}_ids must be int64 [B, L]")
-        if ids.shape[1] > 0 and (ids.stride(1) != 1 or (B > 1 and ids.stride(0) < ids.shape[1])):
-            ids = ids.contiguous()
-        if lens is not None:
-            if lens.dtype != torch.int32 or lens.numel() != B:
-                raise TypeError(f"{name}_lens must be int32 [B]")
-            lens = lens.contiguous()
-        ids_args += [ids, max(ids.stride(0), ids.shape[1]), lens, ids.shape[1]]
-    rows = []
-    for name, x in (("repetition", repetition), ("presence", presence), ("frequency", frequency)):
-        if x is not None:
-            if x.dtype != torch.float32 or x.numel() != B:
-                raise TypeError(f"{name} must be fp32 [B]")
-            x = x.contiguous()
-        rows.append(x)
-    nbias = 0
-    if (bias_ids is None) != (bias is None):
-        raise ValueError("bias_ids and bias go together")
-    if bias_ids is not None:
-        if bias_ids.dtype != torch.int64 or bias_ids.dim() != 2 or bias_ids.shape[0] != B:
-            raise TypeError("bias_ids must be int64 [B, n]")
-        if bias.dtype != torch.float32 or bias.shape != bias_ids.shape:
-            raise TypeError("bias must be fp32 [B, n]")
-        bias_ids, bias = bias_ids.contiguous(), bias.contiguous()
-        nbias = bias_ids.shape[1]
-    allowed_ld = 0
-    if allowed is not None:
-        if allowed.dtype != torch.int32 or allowed.dim() != 2 or allowed.shape[0] != B or allowed.shape[1] * 32 < V:
-            raise TypeError("allowed must be int32 [B, >= ceil(V / 32)]")
-        if allowed.stride(1) != 1 or (B > 1 and allowed.stride(0) < allowed.shape[1]):
-            allowed = allowed.contiguous()
-        allowed_ld = max(allowed.stride(0), allowed.shape[1])
-    _check_status(status)
-    if out is None:
-        out = torch.empty((B, V), dtype=logits.dtype, device=dev)
-    elif (out.shape != (B, V) or out.dtype != logits.dtype or out.stride(1) != 1
-          or (B > 1 and out.stride(0) < V)):
-        raise ValueError("out must be [B, V] of the logits' dtype with unit column stride")
-    if B == 0:
-        return out
-    ld, out_ld = max(logits.stride(0), V), max(out.stride(0), V)
-    with _on(dev):
-        check(
-            lib().lk_process_logits(
-                out.data_ptr(), out_ld, logits.data_ptr(), B, V, ld, _ptr(ids_args[0]), ids_args[1],
-                _ptr(ids_args[2]), ids_args[3], _ptr(ids_args[4]), ids_args[5], _ptr(ids_args[6]),
-                ids_args[7], _ptr(rows[0]), _ptr(rows[1]), _ptr(rows[2]), _ptr(bias_ids),
-                _ptr(bias), nbias, _ptr(allowed), allowed_ld, code, _ptr(status), _stream(dev),
-            )
-        )
-    return out
+    return _spec().logits(logits, prompt_ids, prompt_lens, output_ids, output_lens, repetition,
+                          presence, frequency, bias_ids, bias, allowed, out, status)
 
 
 # ------------------------------------------------ norm + RoPE + KV store ---

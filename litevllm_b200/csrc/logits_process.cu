@@ -13,12 +13,13 @@
 // histories. CTA = (part of the vocabulary, row). Its logits go from global memory
 // through registers and back with the mask applied, a dense pass that knows
 // nothing of tokens; a vector that the mask closes is not read, and in place only
-// closed tokens are written. Meanwhile the CTA counts the row's history tokens of
-// its part in shared memory (so no [B, V] count tensor exists) and lists them, and
-// after the dense pass computes those few tokens, and the biased ones, again from
-// their logits. Reading the counts for every vector instead took 40 us on
-// 128 x 151936 with 16 biases and histories of up to 1024 + 512 tokens (now 26,
-// a bare copy 11).
+// closed tokens are written. Then the CTA counts the row's history tokens of its
+// part in shared memory (so no [B, V] count tensor exists) and lists them, and
+// computes those few tokens, and the biased ones, again from their logits, while
+// other CTAs of the SM are in their dense pass. 128 x 151936 bf16 with 16 biases,
+// masks and histories of up to 1024 + 512 tokens: 24 us (81 MB, 3.4 TB/s; a bare
+// copy 11); with the counts read for every vector it took 40. 8 rows of 128256
+// fp32: 4.9 us, a launch and one CTA's chain of dependent steps.
 // Rows whose addresses are not multiples of 16 bytes keep 16-byte accesses:
 // tokens are indexed from the aligned address in front of the row.
 #include "lk_common.cuh"
@@ -28,7 +29,7 @@ namespace {
 
 constexpr int kLThreads = 256;
 constexpr int kLVecs = 4;        // 16-byte vectors per thread
-constexpr int kLCtas = 5;        // CTAs per SM (4: 28.3 us, 5: 26.5, 6: 28.2 with spills)
+constexpr int kLCtas = 7;        // CTAs per SM (5: 28.0 us, 7: 24.0; with the stores after the history 28.5)
 constexpr int kLMaxBias = 1024;  // bias entries per row
 constexpr int kLList = 2048;     // listed history tokens of a part; more: all counts are looked at
 
@@ -210,49 +211,6 @@ __global__ void __launch_bounds__(kLThreads, kLCtas) logits_process_kernel(const
     }
   }
 
-  // ------------------------------------- the part's history and its biases ---
-  if (sparse) {
-    for (int i = tid; i < CH * C / 128; i += kLThreads)
-      reinterpret_cast<uint4*>(seen)[i] = make_uint4(0u, 0u, 0u, 0u);
-    if (tid == 0) listed = 0;
-    for (int j = tid; j < p.nbias; j += kLThreads) {
-      const int64_t id = p.bias_ids[static_cast<int64_t>(b) * p.nbias + j];
-      if (id >= p.V && p.status && blockIdx.x == 0) atomicOr(p.status, LK_STATUS_TOKEN_OOB);
-      bias_t[j] = id < 0 || id >= p.V ? -1 : static_cast<int>(id);
-      bias_v[j] = p.bias[static_cast<int64_t>(b) * p.nbias + j];
-    }
-    __syncthreads();
-    auto note = [&](int64_t id, bool prompt) {
-      if (id >= p.V && p.status && blockIdx.x == 0) atomicOr(p.status, LK_STATUS_TOKEN_OOB);
-      const int64_t at = id + shift - a0;
-      if (id < 0 || id >= p.V || at < 0 || at >= CH) return;
-      const uint32_t was = prompt ? Mk::set(seen, static_cast<int>(at), Mk::kInPrompt)
-                                  : Mk::count(seen, static_cast<int>(at));
-      if ((was & ~Mk::kBiased) == 0u) {  // its first occurrence
-        const int n = atomicAdd(&listed, 1);
-        if (n < kLList) list[n] = static_cast<uint16_t>(at);
-      }
-    };
-    if (past) {
-      if (p.prompt_ids && r.rep != 1.f) {
-        const int64_t* ids = p.prompt_ids + b * p.prompt_ld;
-        const int n = p.prompt_lens ? min(p.prompt_lens[b], p.prompt_max) : p.prompt_max;
-#pragma unroll 4
-        for (int i = tid; i < n; i += kLThreads) note(__ldg(ids + i), true);
-      }
-      if (p.output_ids) {
-        const int64_t* ids = p.output_ids + b * p.output_ld;
-        const int n = p.output_lens ? min(p.output_lens[b], p.output_max) : p.output_max;
-#pragma unroll 4
-        for (int i = tid; i < n; i += kLThreads) note(__ldg(ids + i), false);
-      }
-    }
-    for (int j = tid; j < p.nbias; j += kLThreads) {
-      const int at = bias_t[j] + shift - a0;
-      if (bias_t[j] >= 0 && at >= 0 && at < CH) Mk::set(seen, at, Mk::kBiased);
-    }
-  }
-
   // ---------------------------------------------------------- dense: stores ---
 #pragma unroll
   for (int k = 0; k < kLVecs; ++k) {
@@ -269,6 +227,47 @@ __global__ void __launch_bounds__(kLThreads, kLCtas) logits_process_kernel(const
     }
   }
   if (!sparse) return;
+
+  // ------------------------------------- the part's history and its biases ---
+  for (int i = tid; i < CH * C / 128; i += kLThreads)
+    reinterpret_cast<uint4*>(seen)[i] = make_uint4(0u, 0u, 0u, 0u);
+  if (tid == 0) listed = 0;
+  for (int j = tid; j < p.nbias; j += kLThreads) {
+    const int64_t id = p.bias_ids[static_cast<int64_t>(b) * p.nbias + j];
+    if (id >= p.V && p.status && blockIdx.x == 0) atomicOr(p.status, LK_STATUS_TOKEN_OOB);
+    bias_t[j] = id < 0 || id >= p.V ? -1 : static_cast<int>(id);
+    bias_v[j] = p.bias[static_cast<int64_t>(b) * p.nbias + j];
+  }
+  __syncthreads();
+  auto note = [&](int64_t id, bool prompt) {
+    if (id >= p.V && p.status && blockIdx.x == 0) atomicOr(p.status, LK_STATUS_TOKEN_OOB);
+    if (id < 0 || id >= p.V) return;
+    const int at = static_cast<int>(id) + shift - a0;
+    if (at < 0 || at >= CH) return;
+    const uint32_t was = prompt ? Mk::set(seen, at, Mk::kInPrompt) : Mk::count(seen, at);
+    if ((was & ~Mk::kBiased) == 0u) {  // its first occurrence
+      const int n = atomicAdd(&listed, 1);
+      if (n < kLList) list[n] = static_cast<uint16_t>(at);
+    }
+  };
+  if (past) {
+    if (p.prompt_ids && r.rep != 1.f) {
+      const int64_t* ids = p.prompt_ids + b * p.prompt_ld;
+      const int n = p.prompt_lens ? min(p.prompt_lens[b], p.prompt_max) : p.prompt_max;
+#pragma unroll 4
+      for (int i = tid; i < n; i += kLThreads) note(__ldg(ids + i), true);
+    }
+    if (p.output_ids) {
+      const int64_t* ids = p.output_ids + b * p.output_ld;
+      const int n = p.output_lens ? min(p.output_lens[b], p.output_max) : p.output_max;
+#pragma unroll 4
+      for (int i = tid; i < n; i += kLThreads) note(__ldg(ids + i), false);
+    }
+  }
+  for (int j = tid; j < p.nbias; j += kLThreads) {
+    const int at = bias_t[j] + shift - a0;
+    if (bias_t[j] >= 0 && at >= 0 && at < CH) Mk::set(seen, at, Mk::kBiased);
+  }
 
   // ---------------------------------- sparse: after the vectors around them ---
   __syncthreads();

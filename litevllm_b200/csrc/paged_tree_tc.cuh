@@ -5,7 +5,7 @@
 //
 // CTA = (128 query rows of one KV head of one sequence, split of its keys), two
 // CTAs per SM, keys in chunks of 64:
-//  * one thread issues S = Q K^T (128 x 64, tcgen05, both operands in shared memory)
+//  * one warp issues S = Q K^T (128 x 64, tcgen05, both operands in shared memory)
 //    into two TMEM buffers in turn and O += P V with P from TMEM, over the first
 //    half of its own S. S of the next chunk is issued before P V of this one, so
 //    the tensor core works during the softmax; the SM's other CTA fills the rest,
@@ -14,12 +14,19 @@
 //    chunk's scores: weights are taken relative to a running maximum that is raised
 //    (and O rescaled in TMEM, the chunk's weights redone) only where one would pass
 //    2^8. Warps whose rows are all padding only keep the barriers going.
-//  * one warp copies K and V, each as its tiles become free, with TMA (boxes of 16
-//    slots through the block table, so block sizes are multiples of 16). 16-bit rows
-//    land in the swizzled operand tiles, two stages deep.
-//  * 8-bit rows land as bytes, V's in the upper half of its operand tile; two warps
-//    for K and two for V take them into registers and widen them to f16 (exactly)
-//    into the operand tiles.
+//  * K and V come with TMA (boxes of 16 slots through the block table, so block sizes
+//    are multiples of 16), two stages deep. 16-bit rows land in the swizzled operand
+//    tiles; a warp waits for K's tiles and another for V's.
+//  * 8-bit rows land as bytes in the upper half of their operand tile; one warp copies
+//    both, looking in turn which tile is free; two warps for K and two for V take the
+//    bytes into registers and widen them to f16 (exactly) into the tile.
+// Latencies bound it, not the tensor pipe (a fifth of the time): a chunk is 3500 cycles
+// from copy to use, 900 S, 1500 the softmax, 900 P V, and two stages in each of two CTAs
+// overlap them to 2300 (16 bits) and 3200 cycles a chunk (8). 32 trees of 20-32 nodes
+// over 64-2048 tokens, bf16, G = 4: 47 us (151 MB, 3.2 TB/s); 16 of 48-64 over 1K-8K,
+// int8: 206 us (330 TFLOP/s). With the bytes of one chunk of K at a time in a buffer of
+// their own the latter took 254, with suspending waits for the copies 230, with one
+// thread alone in the MMA warp's loop 212.
 // Scales as in paged_tree.cuh, but with one running maximum, M, of the weights
 // p s_v: the special-function unit (16 a clock) limits the softmax, so the weight is
 // the product of 2^(x - M), which the denominator sums, and s_v. That costs nothing
@@ -50,24 +57,16 @@ template <int FMT, int D> struct Shape {
   static constexpr int kTHalf = kChunk * 128;
   static constexpr int kT = kHalves * kTHalf;          // operand tile of a K or V chunk
   static constexpr int kRaw = kQ8 ? kChunk * D : 0;    // a chunk's bytes, K or V
-  static constexpr int kSmem = 1024 + kQ + 4 * kT + kRaw;  // two tiles of each, bytes of K
-  // warps: 0-3 softmax; 4-7 widening (8-bit) or 4 looking through V (16-bit); then
-  static constexpr int kMma = kQ8 ? 8 : 5, kCopy = kMma + 1;
-  static constexpr int kThreads = 32 * (kCopy + 1);
+  static constexpr int kSmem = 1024 + kQ + 4 * kT;     // two tiles of each
+  // warps: 0-3 softmax; 8-bit: 4, 5 widening K, 6, 7 V; 16-bit: 4 looking through V;
+  // then one that issues MMAs and one copying (16-bit: one for each of K and V)
+  static constexpr int kMma = kQ8 ? 8 : 5;
+  static constexpr int kThreads = 32 * (kQ8 ? 10 : 8);
 };
 
-// Two lanes of fp32 products per instruction.
-LK_DEVINL void fmul2(float& d0, float& d1, float a0, float a1, float b0, float b1) {
-  asm("{\n\t.reg .b64 ra, rb, rd;\n\t"
-      "mov.b64 ra, {%2, %3};\n\tmov.b64 rb, {%4, %5};\n\t"
-      "mul.rn.f32x2 rd, ra, rb;\n\tmov.b64 {%0, %1}, rd;\n\t}"
-      : "=f"(d0), "=f"(d1)
-      : "f"(a0), "f"(a1), "f"(b0), "f"(b1));
-}
-
 // 8-bit: the softmax takes registers from the widening warps. 128 x kSoftmaxRegs +
-// 128 x kWidenRegs + 64 x 96 stays below the 320 x 96 the CTA is launched with.
-constexpr int kSoftmaxRegs = 120, kWidenRegs = 64;
+// 128 x kWidenRegs + 64 x 96 is the 320 x 96 the CTA is launched with.
+constexpr int kSoftmaxRegs = 120, kWidenRegs = 72;
 template <int N> LK_DEVINL void setmaxnreg_inc() {
   asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
 }
@@ -92,7 +91,7 @@ paged_tree_tc_kernel(const __grid_constant__ CUtensorMap kmap,
   using MT = std::conditional_t<S::kQ8, __half, T>;  // operand type
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2],
-      v_clean[2], s_full[2], p_full[2], o_done[2], sc_full[4], raw_v[2], raw_k, k_taken;
+      v_clean[2], s_full[2], p_full[2], o_done[2], sc_full[4], raw[2][2];
   __shared__ uint32_t tmem_slot;
   __shared__ __align__(16) float s_scale[S::kQ8 ? 4 : 1][2][kChunk];  // s_k, s_v of a chunk
   __shared__ float q_down[kRows];       // 8-bit: what undoes a row's scaling of Q
@@ -102,7 +101,6 @@ paged_tree_tc_kernel(const __grid_constant__ CUtensorMap kmap,
   uint8_t* sQ = smem;
   uint8_t* sK = sQ + S::kQ;               // tile st at st * kT
   uint8_t* sV = sK + 2 * S::kT;
-  uint8_t* staged = sV + 2 * S::kT;       // 8-bit: bytes of a K chunk
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   // Set-up before the wait for the kernel ahead (the store of this step's rows).
@@ -117,10 +115,9 @@ paged_tree_tc_kernel(const __grid_constant__ CUtensorMap kmap,
       mbar_init(&s_full[i], 1);
       mbar_init(&p_full[i], 4);
       mbar_init(&o_done[i], 1);
-      mbar_init(&raw_v[i], 1);
+      mbar_init(&raw[0][i], 1);
+      mbar_init(&raw[1][i], 1);
     }
-    mbar_init(&raw_k, 1);
-    mbar_init(&k_taken, 1);
     for (int i = 0; i < 4; ++i) mbar_init(&sc_full[i], 1);
     fence_barrier_init();
     v_special = 0u;
@@ -165,115 +162,129 @@ paged_tree_tc_kernel(const __grid_constant__ CUtensorMap kmap,
     return !S::kQ8 && (end > open || end > key1);
   };
 
+  // Copies of a warp: chunk k of K or V as TMA boxes of 16 slots. A lane holds the
+  // first slot of one of the boxes of eight chunks, and of the eight after them.
+  const int32_t* bt = p.block_tables + static_cast<int64_t>(b) * p.bt_stride;
+  const int none = max(static_cast<int>(p.num_blocks) * p.bs, 1);  // TMA reads zeros there
+  auto boxes_of = [&](int k0) {
+    const int key = key0 + k0 * kChunk + lane * 16;
+    if (chunks == 0 || key >= key1) return none;
+    const int q = tree_quotient(p, key);
+    const int blk = __ldg(bt + q);
+    if (blk < 0 || blk >= p.num_blocks) {
+      if (p.status) atomicOr(p.status, LK_STATUS_BLOCK_OOB);
+      return none;
+    }
+    return blk * p.bs + (key - q * p.bs);
+  };
+  int boxes[2] = {none, none}, ahead[2] = {none, none};  // K's, V's
+  auto copy = [&](int k, int is_v, const CUtensorMap* map, uint64_t* full, uint8_t* dst) {
+    if ((k & 7) == 0) {
+      boxes[is_v] = k == 0 ? boxes_of(0) : ahead[is_v];
+      ahead[is_v] = boxes_of(k + 8);
+    }
+    int slot[kChunk / 16];
+#pragma unroll
+    for (int i = 0; i < kChunk / 16; ++i)
+      slot[i] = __shfl_sync(0xffffffffu, boxes[is_v], (k & 7) * 4 + i);
+    if (lane == 0) {
+      mbar_arrive_expect_tx(full, S::kQ8 ? S::kRaw : S::kT);
+#pragma unroll
+      for (int i = 0; i < kChunk / 16; ++i) {
+        if constexpr (S::kQ8) {
+          tma_load_3d(dst + i * 16 * D, map, full, 0, slot[i], kvh);
+        } else {
+#pragma unroll
+          for (int c = 0; c < S::kHalves; ++c)
+            tma_load_3d(dst + c * S::kTHalf + i * 2048, map, full, c * 64, slot[i], kvh);
+        }
+      }
+    }
+    __syncwarp();
+  };
+
   if (warp == S::kMma) {
     // ---------------------------------------------------------- MMA issue ---
-    if (lane == 0 && chunks > 0) {
+    if (chunks > 0) {
       constexpr int fmt = std::is_same<MT, __nv_bfloat16>::value ? 1 : 0;
       constexpr uint32_t idS = tc::idesc_f16(fmt, 0, 0, kRows, kChunk);
       constexpr uint32_t idO = tc::idesc_f16(fmt, 0, 1, kRows, D);
-      bool ok = mbar_wait(&q_full, 0);
+      // descriptors differ in their address field alone: bytes / 16
+      const uint64_t dq = tc::smem_desc_sw128(smem_u32(sQ), 16, 1024);
+      const uint64_t dk = tc::smem_desc_sw128(smem_u32(sK), 16, 1024);
+      const uint64_t dv = tc::smem_desc_sw128(smem_u32(sV), S::kTHalf, 1024);
+      bool ok = __all_sync(0xffffffffu, mbar_wait(&q_full, 0));
+      const bool one = tc::elect();  // the thread that issues; all take part in the waits
       auto issue_s = [&](int k) {
         const int st = k & 1;
-        ok = ok && mbar_wait(&k_full[st], (k >> 1) & 1);
+        ok = ok && __all_sync(0xffffffffu, mbar_wait(&k_full[st], (k >> 1) & 1));
         if (!ok) return;
         tc::fence_after();
-        const uint32_t qa = smem_u32(sQ), ka = smem_u32(sK) + st * S::kT;
+        const uint64_t dks = dk + st * (S::kT / 16);
+        if (one) {
 #pragma unroll
-        for (int ks = 0; ks < D / 16; ++ks)
-          tc::mma_f16(tmem + 64 * st,
-                      tc::smem_desc_sw128(qa + (ks >> 2) * S::kQHalf + (ks & 3) * 32, 16, 1024),
-                      tc::smem_desc_sw128(ka + (ks >> 2) * S::kTHalf + (ks & 3) * 32, 16, 1024),
-                      idS, ks > 0 ? 1u : 0u);
-        tc::commit(&s_full[st]);
-        tc::commit(&k_empty[st]);
+          for (int ks = 0; ks < D / 16; ++ks)
+            tc::mma_f16(tmem + 64 * st, dq + ((ks >> 2) * S::kQHalf + (ks & 3) * 32) / 16,
+                        dks + ((ks >> 2) * S::kTHalf + (ks & 3) * 32) / 16, idS, ks > 0 ? 1u : 0u);
+          tc::commit(&s_full[st]);
+          tc::commit(&k_empty[st]);
+        }
+        __syncwarp();
       };
       issue_s(0);
       int cleaned = 0;  // unclean chunks so far
       for (int k = 0; k < chunks && ok; ++k) {
         const int vs = k & 1;
         if (k + 1 < chunks) issue_s(k + 1);  // over S and P of chunk k - 1, whose P V was issued
-        ok = ok && mbar_wait(&v_full[vs], (k >> 1) & 1);
+        ok = ok && __all_sync(0xffffffffu, mbar_wait(&v_full[vs], (k >> 1) & 1));
         if (ok && unclean(k)) {
-          ok = mbar_wait(&v_clean[cleaned & 1], (cleaned >> 1) & 1);
+          ok = __all_sync(0xffffffffu, mbar_wait(&v_clean[cleaned & 1], (cleaned >> 1) & 1));
           ++cleaned;
         }
-        ok = ok && mbar_wait(&p_full[k & 1], (k >> 1) & 1);
+        ok = ok && __all_sync(0xffffffffu, mbar_wait(&p_full[k & 1], (k >> 1) & 1));
         if (!ok) break;
         tc::fence_after();
-        const uint32_t va = smem_u32(sV) + vs * S::kT;
+        const uint64_t dvs = dv + vs * (S::kT / 16);
+        if (one) {
 #pragma unroll
-        for (int kk = 0; kk < kChunk / 16; ++kk)
-          tc::mma_f16_ts(tmem + 128, tmem + 64 * (k & 1) + kk * 8,
-                         tc::smem_desc_sw128(va + kk * 2048, S::kTHalf, 1024), idO,
-                         (k > 0 || kk > 0) ? 1u : 0u);
-        tc::commit(&v_empty[vs]);
-        tc::commit(&o_done[k & 1]);
+          for (int kk = 0; kk < kChunk / 16; ++kk)
+            tc::mma_f16_ts(tmem + 128, tmem + 64 * (k & 1) + kk * 8, dvs + kk * (2048 / 16), idO,
+                           (k > 0 || kk > 0) ? 1u : 0u);
+          tc::commit(&v_empty[vs]);
+          tc::commit(&o_done[k & 1]);
+        }
+        __syncwarp();
       }
-      if (!ok && p.status) atomicOr(p.status, LK_STATUS_WAIT_TIMEOUT);
+      if (!ok && p.status && one) atomicOr(p.status, LK_STATUS_WAIT_TIMEOUT);
     }
-  } else if (warp == S::kCopy) {
+  } else if (warp > S::kMma) {
     // -------------------------------------------------------------- copies ---
+    // 16-bit: a warp waits for the tiles of K, another for V's; 8-bit: one looks at both
+    constexpr bool both = S::kQ8;
+    const bool does_k = both || warp == S::kMma + 1, does_v = both || !does_k;
     if (lane < 2) prefetch_tensormap(lane ? &vmap : &kmap);
-    const int32_t* bt = p.block_tables + static_cast<int64_t>(b) * p.bt_stride;
-    const int none = max(static_cast<int>(p.num_blocks) * p.bs, 1);  // TMA reads zeros there
-    // Slots of the 16-key boxes of eight chunks, one per lane; [0]: K's, [1]: V's, and
-    // the eight chunks after K's.
-    auto boxes_of = [&](int k0) {
-      const int key = key0 + k0 * kChunk + lane * 16;
-      if (chunks == 0 || key >= key1) return none;
-      const int q = tree_quotient(p, key);
-      const int blk = __ldg(bt + q);
-      if (blk < 0 || blk >= p.num_blocks) {
-        if (p.status) atomicOr(p.status, LK_STATUS_BLOCK_OOB);
-        return none;
-      }
-      return blk * p.bs + (key - q * p.bs);
+    int next_k = does_k ? 0 : chunks, next_v = does_v ? 0 : chunks;  // chunks to start
+    auto ready = [&](uint64_t* bar, uint32_t parity) {
+      return both ? mbar_test(bar, parity) : mbar_try_wait(bar, parity);
     };
-    int boxes[2] = {none, none}, ahead = boxes_of(0), last = none;
-    int next[2] = {0, 0};  // chunks to start
-    auto start = [&](int is_v) {
-      const int k = next[is_v]++, st = k & 1;
-      if ((k & 7) == 0) {
-        if (is_v) {
-          boxes[1] = k == 0 || next[0] <= k + 8 ? boxes[0] : last;  // K is at most three ahead
-        } else {
-          last = boxes[0];
-          boxes[0] = ahead;
-          ahead = boxes_of(k + 8);
-        }
-      }
-      const CUtensorMap* map = is_v ? &vmap : &kmap;
-      uint64_t* full = S::kQ8 ? (is_v ? &raw_v[st] : &raw_k) : (is_v ? &v_full[st] : &k_full[st]);
-      uint8_t* dst = S::kQ8 ? (is_v ? sV + st * S::kT + S::kRaw : staged)
-                            : (is_v ? sV : sK) + st * S::kT;
-      if (lane == 0) mbar_arrive_expect_tx(full, S::kQ8 ? S::kRaw : S::kT);
-#pragma unroll
-      for (int i = 0; i < kChunk / 16; ++i) {
-        const int slot = __shfl_sync(0xffffffffu, boxes[is_v], (k & 7) * 4 + i);
-        if (lane == 0) {
-          if constexpr (S::kQ8) {
-            tma_load_3d(dst + i * 16 * D, map, full, 0, slot, kvh);
-          } else {
-#pragma unroll
-            for (int c = 0; c < S::kHalves; ++c)
-              tma_load_3d(dst + c * S::kTHalf + i * 2048, map, full, c * 64, slot, kvh);
-          }
-        }
-      }
-    };
-    // Whichever of K and V has room; K first (S comes before P V).
     uint64_t t0 = globaltimer_ns();
-    while (next[1] < chunks) {
+    while (next_k < chunks || next_v < chunks) {
       bool moved = false;
-      const int kk = next[0], kv = next[1];
-      if (kk < chunks && __all_sync(0xffffffffu, S::kQ8 ? mbar_try_wait(&k_taken, (kk & 1) ^ 1)
-                                                        : mbar_try_wait(&k_empty[kk & 1], ((kk >> 1) & 1) ^ 1))) {
-        start(0);
-        moved = true;
+      if (next_k < chunks) {
+        const int st = next_k & 1;
+        if (__all_sync(0xffffffffu, ready(&k_empty[st], ((next_k >> 1) & 1) ^ 1))) {
+          copy(next_k, 0, &kmap, S::kQ8 ? &raw[0][st] : &k_full[st], sK + st * S::kT + S::kRaw);
+          ++next_k;
+          moved = true;
+        }
       }
-      if (kv < next[0] && __all_sync(0xffffffffu, mbar_try_wait(&v_empty[kv & 1], ((kv >> 1) & 1) ^ 1))) {
-        start(1);
-        moved = true;
+      if (next_v < chunks) {
+        const int st = next_v & 1;
+        if (__all_sync(0xffffffffu, ready(&v_empty[st], ((next_v >> 1) & 1) ^ 1))) {
+          copy(next_v, 1, &vmap, S::kQ8 ? &raw[1][st] : &v_full[st], sV + st * S::kT + S::kRaw);
+          ++next_v;
+          moved = true;
+        }
       }
       if (moved) {
         t0 = globaltimer_ns();
@@ -334,7 +345,14 @@ paged_tree_tc_kernel(const __grid_constant__ CUtensorMap kmap,
       const bool is_v = warp >= 6;
       const int g = threadIdx.x & 63;
       constexpr int kPieces = S::kRaw / 1024;  // 16-byte pieces of a chunk per thread
-      const int32_t* bt = p.block_tables + static_cast<int64_t>(b) * p.bt_stride;
+      // Of a piece, 16 columns c of row r, a thread takes the same c in every (1024 / D)th
+      // row, so its swizzled places are steps of one. In the columns' second half rows
+      // are swapped in pairs: eight lanes write to eight different banks.
+      constexpr int kStep = 1024 / D;
+      const int c = g % (D / 16), r0 = (g / (D / 16)) ^ (c >> 2);
+      const int from = S::kRaw + r0 * D + c * 16;
+      const int to0 = (c >> 2) * S::kTHalf + swz128(r0, (2 * c) & 7);
+      const int to1 = (c >> 2) * S::kTHalf + swz128(r0, (2 * c + 1) & 7);
       // K side: the scales of key g, loaded one chunk ahead, its block two
       int blk = -1;
       float2 cur, nxt = make_float2(0.f, 0.f);
@@ -362,37 +380,33 @@ paged_tree_tc_kernel(const __grid_constant__ CUtensorMap kmap,
           block_at(k + 2);
         }
         const int st = k & 1;
-        uint8_t* dst = (is_v ? sV : sK) + st * S::kT;
-        const uint8_t* raw = is_v ? dst + S::kRaw : staged;
-        ok = is_v ? mbar_wait(&raw_v[st], (k >> 1) & 1) : mbar_wait(&raw_k, k & 1);
+        uint8_t* tile_at = (is_v ? sV : sK) + st * S::kT;
+        ok = mbar_wait(&raw[is_v][st], (k >> 1) & 1);
         uint4 w[kPieces];
         if (ok) {
 #pragma unroll
           for (int i = 0; i < kPieces; ++i)
-            w[i] = reinterpret_cast<const uint4*>(raw)[g + 64 * i];
+            w[i] = *reinterpret_cast<const uint4*>(tile_at + from + i * 1024);
         }
-        // all 64 threads have their bytes: the next K may come, V's tile be written
+        // all 64 threads have their bytes: the tile may be written
         ok = is_v ? named_sync_and(2, 64, ok) : named_sync_and(1, 64, ok);
         if (!ok) break;
-        if (!is_v) {
-          if (g == 0) mbar_arrive(&k_taken);
-          ok = mbar_wait(&k_empty[st], ((k >> 1) & 1) ^ 1);
-        }
-        if (ok) {
+        {
+          const int left = key1 - (key0 + k * kChunk);
+          if (left < kChunk) {  // rows behind the context may hold anything
+#pragma unroll
+            for (int i = 0; i < kPieces; ++i)
+              if (r0 + i * kStep >= left) w[i] = make_uint4(0u, 0u, 0u, 0u);
+          }
 #pragma unroll
           for (int i = 0; i < kPieces; ++i) {
-            const int pc = g + 64 * i;
-            const int r = pc / (D / 16), c = pc % (D / 16);
-            // rows behind the context may hold anything
-            if (key0 + k * kChunk + r >= key1) w[i] = make_uint4(0u, 0u, 0u, 0u);
             uint4 x, y;
             Q8<FMT>::halves(w[i].x, x.x, x.y);
             Q8<FMT>::halves(w[i].y, x.z, x.w);
             Q8<FMT>::halves(w[i].z, y.x, y.y);
             Q8<FMT>::halves(w[i].w, y.z, y.w);
-            uint8_t* base = dst + (c >> 2) * S::kTHalf;  // 16 values: two 16-byte pieces
-            *reinterpret_cast<uint4*>(base + swz128(r, (2 * c) & 7)) = x;
-            *reinterpret_cast<uint4*>(base + swz128(r, (2 * c + 1) & 7)) = y;
+            *reinterpret_cast<uint4*>(tile_at + to0 + i * kStep * 128) = x;
+            *reinterpret_cast<uint4*>(tile_at + to1 + i * kStep * 128) = y;
           }
           if (!is_v) {
             s_scale[k & 3][0][g] = cur.x;

@@ -530,10 +530,15 @@ paged_tree_kernel(const TreeParams p) {
               for (int h = 0; h < 2; ++h) {
                 if (!((window(nt * 8 + 2 * c + h, t0) >> t) & 1u)) continue;
                 const float w = from_16<T>(h ? pw >> 16 : pw & 0xffffu);
+                // the weight is positive even where it is rounded to zero
+                auto part = [&](int d) {
+                  const uint16_t v = vr[at(d)];
+                  return has_special<T>(v) ? from_16<T>(v) : w * from_16<T>(v);
+                };
 #pragma unroll
                 for (int k = 0; k < KS; ++k) {
-                  o[k][nt][h] += w * from_16<T>(vr[at(k * 16 + g)]);
-                  o[k][nt][2 + h] += w * from_16<T>(vr[at(k * 16 + g + 8)]);
+                  o[k][nt][h] += part(k * 16 + g);
+                  o[k][nt][2 + h] += part(k * 16 + g + 8);
                 }
               }
             }

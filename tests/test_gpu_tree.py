@@ -102,7 +102,8 @@ def test_rows_that_see_nothing_are_nan(cuda, kind):
 @pytest.mark.parametrize("value", [float("nan"), float("inf"), -float("inf")])
 @pytest.mark.parametrize("shape", [(8, 2, 128, 16, [50, 37], [9, 20]),
                                    (32, 8, 128, 16, [600, 337], [40, 64]),
-                                   (32, 8, 64, 32, [651, 300], [40, 64])], ids=range(3))
+                                   (32, 8, 64, 32, [651, 300], [40, 64]),
+                                   (32, 8, 128, 16, [600, 337], [9, 20])], ids=range(4))
 def test_special_values_in_hidden_drafts_do_not_leak(cuda, kind, where, value, shape):
     """A drafted token with a NaN or an infinity changes the rows that see it and
     no other."""

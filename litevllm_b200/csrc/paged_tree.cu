@@ -104,11 +104,11 @@ struct Plan {
 // How a call is cut into CTAs, from its sizes alone (contexts are on the device;
 // `keys`, the table's width, bounds them). A unit is (sequence, KV head, group of
 // query rows). Measured on B200, 8 KV heads, G = 4, D = 128, graph-replayed, in us.
-//  * The tcgen05 kernel (128 rows a CTA) where a key row meets enough query rows,
-//    more than 16 of a 16-bit cache or 32 of an 8-bit one (32 rows, 32 x 1000: 16-bit
-//    29 and 35 on mma.sync, int8 41 and 35), and the whole call outweighs its longer
-//    set-up (128 rows, 1 x 4000: 19 and 25; 256 rows, 1 x 256: 15 and 9). Its TMA
-//    boxes want block sizes that are multiples of 16.
+//  * The tcgen05 kernel (128 rows a CTA) where a key row meets more than 16 query rows
+//    (32 x 1000, 24 rows: 16-bit 27 and 33 on mma.sync, int8 32 and 35; 16 rows: 27 and
+//    28, 32 and 25) and the whole call outweighs its longer set-up (1 x 4000, 128 rows:
+//    16 and 28; 8 x 512, 64 rows: 16 and 14; 1 x 256, 256 rows: 12 and 9). Its TMA boxes
+//    want block sizes that are multiples of 16.
 //  * Else NT, the smallest of 1, 2, 4 whose 8 NT rows hold a KV head's, or a smaller
 //    one while its units still leave room on the SMs: a warp with fewer accumulators
 //    is faster, and re-reads come from L2 (16 rows, 8 x 1000: NT 1 13.3, NT 2 13.8;
@@ -118,7 +118,7 @@ struct Plan {
 //    piece 70, 1024 keys 81), and every CTA pays 3 to 4 us of latencies. A piece is at
 //    least 256 keys and at most 1 MB of rows, which a CTA alone on its SM streams in
 //    about 30 us (tcgen05: 2048 keys), so that one long context in a batch does not
-//    outlast the others by more (64 nodes, 16 x 1K-8K, int8: 258, uncut 288).
+//    outlast the others by more (48-64 nodes, 16 x 1K-8K, int8: 206, at 1024 keys 228, at 4096 234).
 //  * Pieces of short contexts (a table of at most 2048 keys) with four or more to a
 //    unit are a cluster, else the workspace and the joining kernel hold them (decode,
 //    1 x 1000: cluster 7.0, joined 7.8, and 5 us less host time for the second launch
@@ -130,7 +130,7 @@ Plan plan_of(int B, int max_q, int H, int H_kv, int D, int fmt, int bs, int max_
   const int64_t heads = static_cast<int64_t>(B) * H_kv;
   const int64_t keys = std::max<int64_t>(1, static_cast<int64_t>(max_blocks) * bs);
   int64_t units = 0, slots = 0;  // resident CTAs
-  if (rows > (fmt == LK_KV_16BIT ? 16 : 32) && bs % 16 == 0 && heads * keys * rows >= (2 << 20)) {
+  if (rows > 16 && bs % 16 == 0 && heads * keys * rows > (2 << 20)) {
     r.NT = 0;
     units = heads * ((rows + 127) / 128);
     slots = 2 * num_sms();

@@ -23,7 +23,7 @@
 // Latencies bound it, not the tensor pipe (a fifth of the time): a chunk is 3500 cycles
 // from copy to use, 900 S, 1500 the softmax, 900 P V, and two stages in each of two CTAs
 // overlap them to 2300 (16 bits) and 3200 cycles a chunk (8). 32 trees of 20-32 nodes
-// over 64-2048 tokens, bf16, G = 4: 47 us (151 MB, 3.2 TB/s); 16 of 48-64 over 1K-8K,
+// over 64-2048 tokens, bf16, G = 4: 46 us (151 MB, 3.3 TB/s); 16 of 48-64 over 1K-8K,
 // int8: 206 us (330 TFLOP/s). With the bytes of one chunk of K at a time in a buffer of
 // their own the latter took 254, with suspending waits for the copies 230, with one
 // thread alone in the MMA warp's loop 212.
@@ -66,7 +66,7 @@ template <int FMT, int D> struct Shape {
 
 // 8-bit: the softmax takes registers from the widening warps. 128 x kSoftmaxRegs +
 // 128 x kWidenRegs + 64 x 96 is the 320 x 96 the CTA is launched with.
-constexpr int kSoftmaxRegs = 120, kWidenRegs = 72;
+constexpr int kSoftmaxRegs = 128, kWidenRegs = 64;
 template <int N> LK_DEVINL void setmaxnreg_inc() {
   asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
 }

@@ -38,6 +38,11 @@ T tensor(PyObject* o, bool optional = false) {
   return &THPVariable_Unpack(o);
 }
 
+int32_t n32(int64_t n) {
+  if (n > INT32_MAX) value_error("a size does not fit 32 bits");
+  return static_cast<int32_t>(n);
+}
+
 int64_t integer(PyObject* o) {
   const long long v = PyLong_AsLongLong(o);
   if (v == -1 && PyErr_Occurred()) throw PyRaised();
@@ -70,7 +75,12 @@ int dtype_code(at::ScalarType t, bool fp32) {
   }
 }
 
-void check(int rc) {
+// Runs a C entry point without the interpreter lock (a launch may wait for room in
+// the queue) and raises its error.
+template <typename... P, typename... A> void call(int (*entry)(P...), A... a) {
+  PyThreadState* state = PyEval_SaveThread();
+  const int rc = entry(a...);
+  PyEval_RestoreThread(state);
   if (rc == LK_OK) return;
   PyErr_Format(g_error, "%s (code %d)", lk_status_string(rc), rc);
   throw PyRaised();
@@ -98,7 +108,9 @@ struct Caches {
   int64_t nb, bs, H_kv, D;
 };
 
-bool is_quantised(PyObject* o) { return PyObject_TypeCheck(o, g_cache_type); }
+bool is_quantised(PyObject* o) {
+  return PyObject_TypeCheck(o, g_cache_type) && PyTuple_GET_SIZE(o) == 2;
+}
 
 Caches caches(PyObject* k, PyObject* v, bool allow_16bit) {
   Caches c = {};
@@ -174,10 +186,10 @@ PyObject* store(PyObject*, PyObject* const* a, Py_ssize_t) {
     check_status(status);
     const at::Tensor s = slots->is_contiguous() ? *slots : slots->contiguous();
     const c10::cuda::CUDAGuard guard(dev);
-    check(lk_store_kv_q8(ptr(key), ptr(value), ptr(c.kd), ptr<float>(c.ks), ptr(c.vd), ptr<float>(c.vs),
-                         static_cast<const int64_t*>(s.data_ptr()), key->size(0), c.H_kv, c.D,
-                         key->stride(0), value->stride(0), c.nb, c.bs, code, c.fmt,
-                         ptr<int32_t>(status), stream_of(dev)));
+    call(lk_store_kv_q8, ptr(key), ptr(value), ptr(c.kd), ptr<float>(c.ks), ptr(c.vd),
+         ptr<float>(c.vs), static_cast<const int64_t*>(s.data_ptr()), n32(key->size(0)), n32(c.H_kv),
+         n32(c.D), key->stride(0), value->stride(0), c.nb, n32(c.bs), code, c.fmt,
+         ptr<int32_t>(status), stream_of(dev));
     Py_RETURN_NONE;
   });
 }
@@ -217,10 +229,10 @@ PyObject* load(PyObject*, PyObject* const* a, Py_ssize_t) {
           value_error("key_out/value_out must be contiguous [num_rows, H_kv, D] of dtype");
       }
     }
-    check(lk_load_kv_q8(outs[0].data_ptr(), outs[1].data_ptr(), ptr(c.kd), ptr<float>(c.ks), ptr(c.vd),
-                        ptr<float>(c.vs), ptr<int32_t>(bt), bt->stride(0), ptr<int32_t>(ctx),
-                        ptr<int32_t>(cu), B, rows, c.H_kv, c.D, c.nb, c.bs, max_blocks, code, c.fmt,
-                        ptr<int32_t>(status), stream_of(dev)));
+    call(lk_load_kv_q8, outs[0].data_ptr(), outs[1].data_ptr(), ptr(c.kd), ptr<float>(c.ks),
+         ptr(c.vd), ptr<float>(c.vs), ptr<int32_t>(bt), bt->stride(0), ptr<int32_t>(ctx),
+         ptr<int32_t>(cu), n32(B), rows, n32(c.H_kv), n32(c.D), c.nb, n32(c.bs), n32(max_blocks),
+         code, c.fmt, ptr<int32_t>(status), stream_of(dev));
     PyObject* t = PyTuple_New(2);
     if (!t) throw PyRaised();
     for (int i = 0; i < 2; ++i) {
@@ -252,7 +264,6 @@ PyObject* tree(PyObject*, PyObject* const* a, Py_ssize_t) {
     if (bt->scalar_type() != at::kInt || bt->dim() != 2) type_error("block_tables must be int32 [B, max_blocks]");
     const int64_t B = bt->size(0), max_blocks = bt->size(1), max_q = decode ? 1 : integer(a[6]);
     if (max_q < 0) value_error("max_q_len must not be negative");
-    if (max_q > INT32_MAX || n > INT32_MAX) value_error("too many query tokens");
     if (decode && B != n) value_error("decode takes one query per row of block_tables");
     at::Tensor bt_keep, ctx_keep, cu_keep, mask_keep;
     if (max_blocks > 0 && bt->stride(1) != 1) {
@@ -289,7 +300,8 @@ PyObject* tree(PyObject*, PyObject* const* a, Py_ssize_t) {
     if (n == 0 || B == 0 || max_q == 0) return result();
     // The partials of split contexts live in a buffer of this call's own unless the
     // caller gives one: calls on other streams and captured graphs never share it.
-    const size_t need = lk_paged_tree_workspace_bytes(n, B, max_q, H, c.H_kv, D, c.bs, max_blocks, c.fmt);
+    const size_t need = lk_paged_tree_workspace_bytes(n32(n), n32(B), n32(max_q), n32(H), n32(c.H_kv),
+                                                      n32(D), n32(c.bs), n32(max_blocks), c.fmt);
     at::Tensor ws;
     void* ws_ptr = nullptr;
     size_t ws_bytes = 0;
@@ -305,11 +317,12 @@ PyObject* tree(PyObject*, PyObject* const* a, Py_ssize_t) {
       ws_ptr = ws.data_ptr();
       ws_bytes = need;
     }
-    check(lk_paged_tree_attention(
-        out.data_ptr(), out.stride(0), ptr(query), query->stride(0), ptr(c.kd), ptr<float>(c.ks), ptr(c.vd),
-        ptr<float>(c.vs), c.nb, ptr<int32_t>(bt), bt->stride(0), ptr<int32_t>(cu), ptr<int32_t>(ctx),
-        ptr<int64_t>(mask), mask ? mask->stride(0) : 0, mask ? mask->size(1) : 0, n, B, max_q, H, c.H_kv, D,
-        c.bs, max_blocks, scale, code, c.fmt, ws_ptr, ws_bytes, ptr<int32_t>(status), stream_of(dev)));
+    call(lk_paged_tree_attention, out.data_ptr(), out.stride(0), ptr(query), query->stride(0),
+         ptr(c.kd), ptr<float>(c.ks), ptr(c.vd), ptr<float>(c.vs), c.nb, ptr<int32_t>(bt),
+         bt->stride(0), ptr<int32_t>(cu), ptr<int32_t>(ctx), ptr<int64_t>(mask),
+         mask ? mask->stride(0) : 0, mask ? n32(mask->size(1)) : 0, n32(n), n32(B), n32(max_q), n32(H),
+         n32(c.H_kv), n32(D), n32(c.bs), n32(max_blocks), static_cast<float>(scale), code, c.fmt,
+         ws_ptr, ws_bytes, ptr<int32_t>(status), stream_of(dev));
     return result();
   });
 }
@@ -385,12 +398,11 @@ PyObject* logits(PyObject*, PyObject* const* a, Py_ssize_t) {
         value_error("out must be [B, V] of the logits' dtype with unit column stride");
     }
     if (B > 0)
-      check(lk_process_logits(
-          out.data_ptr(), std::max(out.stride(0), V), ptr(x), B, V, ld(x), ptr<int64_t>(p), ld(p),
-          ptr<int32_t>(pl), p ? p->size(1) : 0, ptr<int64_t>(o), ld(o), ptr<int32_t>(ol),
-          o ? o->size(1) : 0, ptr<float>(term[0]), ptr<float>(term[1]), ptr<float>(term[2]),
-          ptr<int64_t>(bi), ptr<float>(bv), bi ? bi->size(1) : 0, ptr<int32_t>(al), ld(al), code,
-          ptr<int32_t>(status), stream_of(dev)));
+      call(lk_process_logits, out.data_ptr(), std::max(out.stride(0), V), ptr(x), n32(B), n32(V),
+           ld(x), ptr<int64_t>(p), ld(p), ptr<int32_t>(pl), p ? n32(p->size(1)) : 0, ptr<int64_t>(o),
+           ld(o), ptr<int32_t>(ol), o ? n32(o->size(1)) : 0, ptr<float>(term[0]), ptr<float>(term[1]),
+           ptr<float>(term[2]), ptr<int64_t>(bi), ptr<float>(bv), bi ? n32(bi->size(1)) : 0,
+           ptr<int32_t>(al), ld(al), code, ptr<int32_t>(status), stream_of(dev));
     return out_in ? Py_NewRef(a[11]) : THPVariable_Wrap(out);
   });
 }

@@ -3,13 +3,15 @@
 rows, ragged batches, splits, streams and captured graphs."""
 
 import random
+import types
 
 import pytest
 import torch
 
-from litevllm_b200 import _lib, ops
+from litevllm_b200 import _lib, model_hooks, ops
 from litevllm_b200.attention import Attention
 from litevllm_b200.sampler import Sampler
+from oracle import kv_q8
 from oracle import logits as olog
 from oracle import tree_attention
 from tests.spec_inputs import (EPS, assert_attention, bits_of, cache_for, on, randn, random_tree,
@@ -361,3 +363,46 @@ def test_mixed_step_over_an_8bit_cache(cuda, kind):
                              torch.tensor([0, 20], dtype=torch.int32).cuda(), 1, 20, 20)
     want, size = tree_attention.tree(q, kd, ks, vd, vs, tables, ctx, q_lens, [None] * 3, attn.scale)
     assert (got.double().cpu() - want).abs().max() <= 2 ** -8 * want.abs().max() + 16 * 2 ** -8 * size.max()
+
+
+@pytest.mark.parametrize("kind", [INT8, E4M3])
+def test_fused_block_writes_and_reads_an_8bit_cache(cuda, kind):
+    """The fused attention block over an 8-bit cache: it holds the rows that the
+    16-bit cache gets, quantised, and a decode step attends to them."""
+    H, H_kv, D, bs, hidden, S = 8, 2, 128, 16, 64, 21
+    dev = dict(device=cuda, dtype=BF16)
+    m = types.SimpleNamespace(num_heads=H, num_kv_heads=H_kv, head_dim=D, o_proj=lambda x: x)
+    for i, (name, n) in enumerate((("q_proj", H), ("k_proj", H_kv), ("v_proj", H_kv))):
+        w = randn(40 + i, hidden, n * D, dtype=BF16).to(cuda)
+        setattr(m, name, lambda x, w=w: x @ w)
+    angle = torch.arange(64, device=cuda)[:, None] * 0.01 * torch.arange(D // 2, device=cuda)
+    m.rotary_emb = types.SimpleNamespace(cos_cached=angle.cos(), sin_cached=angle.sin())
+    queries = []
+
+    class Recording(Attention):
+        def forward(self, query, *args, **kw):
+            queries.append(query.clone())
+            return super().forward(query, *args, **kw)
+
+    m.attn = Recording(H, D, H_kv)
+    x = randn(44, S + 1, hidden, dtype=BF16).to(cuda)
+    pos, slots = torch.arange(S + 1, device=cuda), torch.arange(16, S + 17, device=cuda)
+    table = torch.tensor([[1, 2]], dtype=torch.int32, device=cuda)
+    out = {}
+    for cache in ("16", "8"):
+        kc, vc = ([torch.zeros(4, bs, H_kv, D, **dev) for _ in range(2)] if cache == "16" else
+                  [ops.new_quantized_cache(4, bs, H_kv, D, kind, device=cuda) for _ in range(2)])
+        for rows, prefill in ((slice(0, S), True), (slice(S, S + 1), False)):
+            y = model_hooks.fused_forward(
+                m, x[rows], pos[rows], (kc, vc), slots[rows], None if prefill else table,
+                None if prefill else torch.tensor([S + 1], dtype=torch.int32, device=cuda), prefill)
+        out[cache] = kc, vc, y
+    for wide, (data, scale) in zip(out["16"][:2], out["8"][:2]):
+        q, s = kv_q8.quantise(wide.view(-1, H_kv, D)[16:S + 17].cpu(), kind)
+        assert torch.equal(data.view(-1, H_kv, D)[16:S + 17].float().cpu().double(), q)
+        assert torch.equal(scale.transpose(1, 2).reshape(-1, H_kv)[16:S + 17].cpu(), s)
+    (kd, ks), (vd, vs), y = out["8"]
+    kd, ks, vd, vs = (t.cpu() for t in (kd, ks, vd, vs))
+    q = queries[-1].cpu()
+    want, size = tree_attention.tree(q, kd, ks, vd, vs, table.cpu(), [S + 1], [1], [None], m.attn.scale)
+    assert_attention(y.view(1, H, D), want, size, q, row_bounds(kd, ks, vd, vs), m.attn.scale, S + 1, EPS[F16])

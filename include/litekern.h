@@ -361,8 +361,8 @@ int lk_paged_decode_q8(void* out, int64_t out_token_stride, const void* q, int64
  * Any of the operands may be NULL (off). prompt_ids / output_ids: int64
  * [B, prompt_max] / [B, output_max] with row strides, of which the first
  * prompt_lens[b] / output_lens[b] count (NULL: all); a negative id is padding,
- * an id >= V is skipped and flagged LK_STATUS_TOKEN_OOB in *status (may be
- * NULL). bias_ids int64 / bias fp32: [B, num_bias] contiguous, num_bias <= 1024, ids
+ * an id >= V is skipped and, in a list that one of the row's penalties needs,
+ * flagged LK_STATUS_TOKEN_OOB in *status (may be NULL). bias_ids int64 / bias fp32: [B, num_bias] contiguous, num_bias <= 1024, ids
  * as above. allowed: int32 words, row stride allowed_ld. logits / out: [B, V],
  * F32, F16 or BF16, row strides ld / out_ld; out may be logits (the same ld),
  * and otherwise must not overlap it. B <= 65535.

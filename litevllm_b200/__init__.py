@@ -5,7 +5,8 @@
 
 Modules: ops (C-ABI wrappers), attention (drop-in Attention / PagedAttention),
 sampler (drop-in Sampler), workloads (seeded synthetic inputs), sharding
-(request sharding across GPUs), build (nvcc build of liblitekern.so).
+(request sharding across GPUs), build (nvcc build of liblitekern.so, g++ build of
+its native binding _spec.so).
 """
 
 from __future__ import annotations

@@ -16,6 +16,7 @@ struct JoinParams {
   const float* part_o;    // [T * H][nsplit][D]
   const int32_t* cu_seqlens_q;
   const int32_t* context_lens;
+  uint32_t rows;  // T * H
   int B, H, nsplit, chunk, max_keys, max_q;
 };
 
@@ -24,13 +25,15 @@ template <> LK_DEVINL __nv_bfloat16 join_round<__nv_bfloat16>(float x) { return 
 template <> LK_DEVINL __half join_round<__half>(float x) { return __float2half_rn(x); }
 
 // out = sum_s O_s 2^(M_s - M) / sum_s l_s 2^(m_s - m) * 2^(M - m), in split
-// order whatever order the splits ended in. One CTA per query row; W warps
-// share its splits (few splits: one warp, many rows; many: four).
+// order whatever order the splits ended in. Four warps: a query row each where rows
+// are many and splits few (29K rows of up to four: 17 us from a cold cache, 21 with a
+// CTA per row), else all four on one row, W = 4 (256 rows of up to eight: 7.0 and 9.5).
 template <typename T, int D, int W>
-__global__ void __launch_bounds__(W * 32) tree_join_kernel(const JoinParams p) {
+__global__ void __launch_bounds__(128) tree_join_kernel(const JoinParams p) {
   pdl_wait();
-  const int64_t row = blockIdx.x;
-  const int t = static_cast<int>(row / p.H), h = static_cast<int>(row % p.H);
+  const uint32_t row = W > 1 ? blockIdx.x : blockIdx.x * 4u + (threadIdx.x >> 5);  // < 2^31 + 4
+  if (row >= p.rows) return;
+  const int t = row / static_cast<uint32_t>(p.H), h = row - t * static_cast<uint32_t>(p.H);
   int b = t;
   if (p.cu_seqlens_q) {
     if (t < p.cu_seqlens_q[0] || t >= p.cu_seqlens_q[p.B]) return;
@@ -46,8 +49,8 @@ __global__ void __launch_bounds__(W * 32) tree_join_kernel(const JoinParams p) {
   const int ctx = max(min(p.context_lens[b], p.max_keys), 0);
   const int ns = (ctx + p.chunk - 1) / p.chunk;
   if (ns <= 1) return;  // written by its only split
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const float4* ml = p.part_ml + row * p.nsplit;
+  const int warp = W > 1 ? threadIdx.x >> 5 : 0, lane = threadIdx.x & 31;
+  const float4* ml = p.part_ml + static_cast<int64_t>(row) * p.nsplit;
   float a = -3.402823466e38f, A = a;
   for (int s = lane; s < ns; s += 32) {
     const float4 w = ml[s];
@@ -65,13 +68,12 @@ __global__ void __launch_bounds__(W * 32) tree_join_kernel(const JoinParams p) {
     const float4 w = ml[s];
     const float f = ex2_mufu(w.z - A);
     L += w.y * ex2_mufu(w.x - a);
-    const float* po = p.part_o + (row * p.nsplit + s) * D + lane * V;
+    const float* po = p.part_o + (static_cast<int64_t>(row) * p.nsplit + s) * D + lane * V;
+    __align__(16) float x[V];
+    if constexpr (V == 4) *reinterpret_cast<float4*>(x) = *reinterpret_cast<const float4*>(po);
+    else *reinterpret_cast<float2*>(x) = *reinterpret_cast<const float2*>(po);
 #pragma unroll
-    for (int i = 0; i < V; i += 2) {
-      const float2 x = *reinterpret_cast<const float2*>(po + i);
-      acc[i] += x.x * f;
-      acc[i + 1] += x.y * f;
-    }
+    for (int i = 0; i < V; ++i) acc[i] += x[i] * f;
   }
   if constexpr (W > 1) {
     __shared__ float sm[W][D + 1];
@@ -118,7 +120,7 @@ struct Plan {
 //    piece 70, 1024 keys 81), and every CTA pays 3 to 4 us of latencies. A piece is at
 //    least 256 keys and at most 1 MB of rows, which a CTA alone on its SM streams in
 //    about 30 us (tcgen05: 2048 keys), so that one long context in a batch does not
-//    outlast the others by more (48-64 nodes, 16 x 1K-8K, int8: 206, at 1024 keys 228, at 4096 234).
+//    outlast the others by more (48-64 nodes, 16 x 1K-8K, int8: 206 then, at 1024 keys 228, at 4096 234).
 //  * Pieces of short contexts (a table of at most 2048 keys) with four or more to a
 //    unit are a cluster, else the workspace and the joining kernel hold them (decode,
 //    1 x 1000: cluster 7.0, joined 7.8, and 5 us less host time for the second launch
@@ -169,8 +171,8 @@ size_t plan_bytes(const Plan& r, int64_t T, int H, int D) {
 
 template <typename T, int D>
 cudaError_t join(const JoinParams& j, unsigned rows, cudaStream_t s) {
-  if (j.nsplit <= 8)
-    return launch_after_previous(tree_join_kernel<T, D, 1>, dim3(rows), dim3(32), 0, s, j);
+  if (j.nsplit <= 8 && rows > 2048)
+    return launch_after_previous(tree_join_kernel<T, D, 1>, dim3((rows + 3) / 4), dim3(128), 0, s, j);
   return launch_after_previous(tree_join_kernel<T, D, 4>, dim3(rows), dim3(128), 0, s, j);
 }
 
@@ -214,6 +216,7 @@ int run(TreeParams& p, int T, int H, int D, float scale, int dtype, int fmt, voi
   j.part_o = p.part_o;
   j.cu_seqlens_q = p.cu_seqlens_q;
   j.context_lens = p.context_lens;
+  j.rows = static_cast<uint32_t>(T) * H;
   j.B = p.B;
   j.H = H;
   j.nsplit = r.nsplit;

@@ -24,7 +24,7 @@
 // from copy to use, 900 S, 1500 the softmax, 900 P V, and two stages in each of two CTAs
 // overlap them to 2300 (16 bits) and 3200 cycles a chunk (8). 32 trees of 20-32 nodes
 // over 64-2048 tokens, bf16, G = 4: 46 us (151 MB, 3.3 TB/s); 16 of 48-64 over 1K-8K,
-// int8: 206 us (330 TFLOP/s). With the bytes of one chunk of K at a time in a buffer of
+// int8: 201 us with the join (337 TFLOP/s). With the bytes of one chunk of K at a time in a buffer of
 // their own the latter took 254, with suspending waits for the copies 230, with one
 // thread alone in the MMA warp's loop 212.
 // Scales as in paged_tree.cuh, but with one running maximum, M, of the weights

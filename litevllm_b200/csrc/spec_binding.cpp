@@ -229,6 +229,8 @@ PyObject* load(PyObject*, PyObject* const* a, Py_ssize_t) {
           value_error("key_out/value_out must be contiguous [num_rows, H_kv, D] of dtype");
       }
     }
+    if (ko && vo && rows > 0 && ko->data_ptr() == vo->data_ptr())
+      value_error("key_out and value_out must be different tensors");
     call(lk_load_kv_q8, outs[0].data_ptr(), outs[1].data_ptr(), ptr(c.kd), ptr<float>(c.ks),
          ptr(c.vd), ptr<float>(c.vs), ptr<int32_t>(bt), bt->stride(0), ptr<int32_t>(ctx),
          ptr<int32_t>(cu), n32(B), rows, n32(c.H_kv), n32(c.D), c.nb, n32(c.bs), n32(max_blocks),
@@ -293,7 +295,7 @@ PyObject* tree(PyObject*, PyObject* const* a, Py_ssize_t) {
     } else {
       out = *out_in;
       if (out.dim() != 3 || out.sizes() != query->sizes() || out.scalar_type() != query->scalar_type() ||
-          out.stride(2) != 1 || out.stride(1) != D)
+          out.stride(2) != 1 || out.stride(1) != D || (n > 1 && out.stride(0) < H * D))
         value_error("bad out tensor");
     }
     auto result = [&]() { return out_in ? Py_NewRef(a[9]) : THPVariable_Wrap(out); };
@@ -306,6 +308,7 @@ PyObject* tree(PyObject*, PyObject* const* a, Py_ssize_t) {
     void* ws_ptr = nullptr;
     size_t ws_bytes = 0;
     if (ws_in) {
+      if (!ws_in->is_contiguous()) value_error("workspace must be contiguous");
       ws_ptr = ws_in->data_ptr();
       ws_bytes = ws_in->nbytes();
       if (ws_bytes < need) {

@@ -168,6 +168,8 @@ DECODE = [  # (H, H_kv, D, bs, ctx)
     (40, 1, 64, 32, [100, 513]),                              # G = 40
     (14, 2, 128, 48, [2500, 40]),                             # G = 7
     (5, 5, 64, 1, [66, 3]),                                   # one-slot blocks
+    (80, 2, 128, 16, [4097, 0, 1, 2500, 64, 63, 3000]),       # G = 40, enough work for tcgen05
+    (128, 1, 64, 32, [4097, 4096, 4000, 65, 4095]),           # G = 128, the same
 ]
 
 

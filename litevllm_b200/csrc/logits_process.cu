@@ -287,12 +287,15 @@ __global__ void __launch_bounds__(kLThreads, kLCtas) logits_process_kernel(const
     const int v = bias_t[j];
     const int at = v + shift - a0;
     if (v < 0 || at < 0 || at >= CH || !is_open(v)) continue;
-    bool first = true;  // the first entry of a token adds up all of them
-    for (int i = 0; i < j && first; ++i) first = bias_t[i] != v;
-    if (!first) continue;
+    bool first = true;  // the first entry of a token adds up all of them, in list order
     float sum = 0.f;
-    for (int i = j; i < p.nbias; ++i)
-      if (bias_t[i] == v) sum = __fadd_rn(sum, bias_v[i]);
+#pragma unroll 8
+    for (int i = 0; i < p.nbias; ++i) {
+      const bool same = bias_t[i] == v;
+      first &= !same || i >= j;
+      sum = same ? __fadd_rn(sum, bias_v[i]) : sum;
+    }
+    if (!first) continue;
     out[v] = Raw<T>::round(__fadd_rn(process<C>(lk::Elem<T>::to_f(in[v]), Mk::get(seen, at), r), sum));
   }
 }

@@ -250,6 +250,7 @@ PyObject* load(PyObject*, PyObject* const* a, Py_ssize_t) {
 PyObject* tree(PyObject*, PyObject* const* a, Py_ssize_t) {
   return guarded([&]() -> PyObject* {
     const bool decode = a[6] == Py_None;
+    if (decode && a[5] != Py_None) type_error("max_q_len must be an integer");
     const Caches c = caches(a[1], a[2], !decode);
     const T query = tensor(a[0]), mask_in = tensor(a[8], true), out_in = tensor(a[9], true);
     T bt = tensor(a[3]), ctx = tensor(a[4]), cu = tensor(a[5], decode);

@@ -76,6 +76,7 @@ def test_attention(cuda):
     refused(TypeError, "cu_seqlens_q", f, args, cu_seqlens_q=i32(0, 1, 3))
     refused(TypeError, "Tensor", f, args, cu_seqlens_q=None)
     refused(ValueError, "max_q_len", f, args, max_q_len=-1)
+    refused(TypeError, "max_q_len", f, args, max_q_len=None)
     refused(TypeError, "tree_mask", f, args, tree_mask=mask.int())
     refused(TypeError, "tree_mask", f, args, tree_mask=mask[:2])
     refused(ValueError, "tree_mask", f, args, max_q_len=65)

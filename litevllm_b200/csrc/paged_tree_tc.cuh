@@ -753,6 +753,11 @@ int launch(const TreeParams& p, unsigned grid, cudaStream_t s) {
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) !=
         cudaSuccess)
       return LK_ERR_CUDA;
+    if (Shape<FMT, D>::kQ8) {  // a build whose registers do not add up must not wait for them
+      cudaFuncAttributes a;
+      if (cudaFuncGetAttributes(&a, kernel) != cudaSuccess) return LK_ERR_CUDA;
+      if (128 * (kSoftmaxRegs + kWidenRegs) > 256 * a.numRegs) return LK_ERR_UNSUPPORTED;
+    }
     if (dev < 64) ready.fetch_or(bit, std::memory_order_relaxed);
   }
   CUtensorMap km, vm;

@@ -122,7 +122,10 @@ paged_tree_tc_kernel(const __grid_constant__ CUtensorMap kmap,
     fence_barrier_init();
     v_special = 0u;
   }
-  if (warp == S::kMma) tc::alloc(&tmem_slot, 256);
+  if (warp == S::kMma) {
+    __syncwarp();
+    tc::alloc(&tmem_slot, 256);
+  }
   tc::fence_before();
   __syncthreads();
   tc::fence_after();
@@ -341,6 +344,7 @@ paged_tree_tc_kernel(const __grid_constant__ CUtensorMap kmap,
       }
     } else {
       // ------------------------------------------------------ 8-bit widening ---
+      __syncwarp();  // all 32 lanes issue it together
       setmaxnreg_dec<kWidenRegs>();
       const bool is_v = warp >= 6;
       const int g = threadIdx.x & 63;
@@ -425,6 +429,10 @@ paged_tree_tc_kernel(const __grid_constant__ CUtensorMap kmap,
     if (!ok && p.status && lane == 0) atomicOr(p.status, LK_STATUS_WAIT_TIMEOUT);
   } else {
     // ------------------------------------------------------------- softmax ---
+    // Waits, masks and special values part the lanes of a warp: before each of the
+    // instructions that all 32 have to issue together (register split, TMEM loads and
+    // stores) they are brought together again.
+    __syncwarp();
     if constexpr (S::kQ8) setmaxnreg_inc<kSoftmaxRegs>();
    if (live) {
     const int t = threadIdx.x;                           // row of the CTA
@@ -562,6 +570,7 @@ paged_tree_tc_kernel(const __grid_constant__ CUtensorMap kmap,
 #pragma unroll 1
             for (int c = 0; c < 2; ++c) {
               uint32_t sv[32];
+              __syncwarp();
               tc::ld32(tS + 32 * c, sv);
               tc::wait_ld();
               const uint32_t seen = static_cast<uint32_t>(bits >> (32 * c));
@@ -580,7 +589,8 @@ paged_tree_tc_kernel(const __grid_constant__ CUtensorMap kmap,
             if (k > 0) {
               // O is stable once P V of chunk k - 1 has completed; P V of chunk k
               // waits for this warp's P
-              if (!mbar_wait(&o_done[(k - 1) & 1], ((k - 1) >> 1) & 1)) ok = false;
+              ok = __all_sync(0xffffffffu, mbar_wait(&o_done[(k - 1) & 1], ((k - 1) >> 1) & 1));
+              if (!ok) break;
               tc::fence_after();
 #pragma unroll 1
               for (int c = 0; c < D / 32; ++c) {
@@ -598,6 +608,7 @@ paged_tree_tc_kernel(const __grid_constant__ CUtensorMap kmap,
           sum0 = sum1 = 0.f;
           auto weigh = [&](auto with_mask) {
             uint32_t sv[64];
+            __syncwarp();
             tc::ld32(tS, *reinterpret_cast<uint32_t(*)[32]>(sv));
             tc::ld32(tS + 32, *reinterpret_cast<uint32_t(*)[32]>(sv + 32));
             tc::wait_ld();
@@ -648,9 +659,9 @@ paged_tree_tc_kernel(const __grid_constant__ CUtensorMap kmap,
           raise = __any_sync(0xffffffffu, up);
           if (!raise) break;
         }
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
+        if (!ok) break;  // alike in all lanes
         l += sum0 + sum1;
+        __syncwarp();
         tc::st32(tS, pw);
         tc::wait_st();
         tc::fence_before();
@@ -681,6 +692,7 @@ paged_tree_tc_kernel(const __grid_constant__ CUtensorMap kmap,
       for (int c = 0; c < D / 32; ++c) {
         uint32_t ov[32];
         if (chunks > 0) {
+          __syncwarp();  // lanes part below
           tc::ld32(tO + lanes + 32 * c, ov);
           tc::wait_ld();
         } else {
@@ -705,8 +717,7 @@ paged_tree_tc_kernel(const __grid_constant__ CUtensorMap kmap,
             }
           }
         }
-        if (!row_ok) continue;
-        if (whole) {
+        if (row_ok && whole) {
 #pragma unroll
           for (int i = 0; i < 32; i += 8) {
             uint32_t w[4];
@@ -723,7 +734,7 @@ paged_tree_tc_kernel(const __grid_constant__ CUtensorMap kmap,
                 o16[e] = static_cast<uint16_t>(w[e >> 1] >> ((e & 1) * 16));
             }
           }
-        } else {
+        } else if (row_ok) {
           float4* po = reinterpret_cast<float4*>(p.part_o + part * D + 32 * c);
 #pragma unroll
           for (int i = 0; i < 8; ++i)
@@ -738,6 +749,7 @@ paged_tree_tc_kernel(const __grid_constant__ CUtensorMap kmap,
   tc::fence_before();
   __syncthreads();
   tc::fence_after();
+  __syncwarp();
   if (warp == S::kMma) tc::dealloc(tmem, 256);
 }
 

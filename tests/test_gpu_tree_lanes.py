@@ -1,0 +1,72 @@
+"""Drafted-tree attention where the query rows of one warp go different ways: rows
+whose largest score comes late and not in the same place, row counts that fill no
+whole warp, and special values that only some rows see."""
+
+import random
+
+import pytest
+import torch
+
+from oracle import kv_q8
+from tests.test_gpu_tree import BF16, E4M3, F16, INT8, case, check, run
+
+pytestmark = pytest.mark.gpu
+
+
+def put_row(c, which, b, key, rows):
+    """Rows [H_kv, D] as the K or V (which) of one position of sequence b."""
+    bs = c["kd"].shape[1]
+    blk, off = c["tables"][b, key // bs], key % bs
+    if c["ks"] is None:
+        c[which + "d"][blk, off] = rows.to(c["kd"].dtype)
+    else:
+        q, s = kv_q8.quantise(rows.to(c["q"].dtype), c["kd"].dtype)
+        c[which + "d"][blk, off] = q.float().to(c["kd"].dtype)
+        c[which + "s"][blk, :, off] = s
+
+
+def late_maxima(kind, counts, seed, tables_to=256):
+    """Contexts of some 700 keys under a wide table (many keys for one CTA of the
+    tcgen05 kernel), where a key in each 64 points along one query row, ever
+    longer: that row's maximum rises there, and others' where they lie near it."""
+    rng = random.Random(seed)
+    dtype = kind if kind in (BF16, F16) else BF16
+    H, H_kv, D = 32, 8, 128
+    ctx = [rng.randint(640, 740) for _ in counts]
+    c = case(kind, dtype, H, H_kv, D, 16, ctx, counts, seed=seed)
+    extra = tables_to - c["tables"].shape[1]
+    c["tables"] = torch.cat([c["tables"], torch.zeros((len(ctx), extra), dtype=torch.int32)], 1)
+    at = 0
+    for b, n in enumerate(counts):
+        for j in range((ctx[b] - n) // 64):
+            token = at + rng.randrange(n)
+            q = c["q"][token].float().view(H_kv, H // H_kv, D)[:, rng.randrange(H // H_kv)]
+            put_row(c, "k", b, 64 * j + rng.randrange(64), q / q.norm(dim=-1, keepdim=True) * 9.0 * (j + 1))
+        at += n
+    return c
+
+
+@pytest.mark.parametrize("kind", [BF16, F16, INT8, E4M3])
+@pytest.mark.parametrize("counts", [[5, 9, 13, 7, 1, 11, 8, 10, 3, 12, 6, 13], [33, 40, 17, 64] * 3],
+                         ids=["one tile", "two tiles"])
+def test_maxima_that_rise_late(cuda, kind, counts):
+    c = late_maxima(kind, counts, seed=len(set(counts)))
+    status = torch.zeros(1, dtype=torch.int32, device=cuda)
+    got = run(c, cuda, status=status)
+    check(c, got)
+    assert status.item() == 0
+    assert all(torch.equal(got, run(c, cuda)) for _ in range(3))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_special_values_beside_rows_that_fill_no_warp(cuda, dtype):
+    """Drafted V rows with infinities, seen by some of 36 to 52 query rows."""
+    counts = [13, 9, 11] * 4
+    c = late_maxima(dtype, counts, seed=5)
+    for b, n in enumerate(counts):
+        rows = torch.ones((8, 128))
+        rows[:, 70 + b] = float("inf")
+        put_row(c, "v", b, c["ctx"][b] - n + 2, rows)
+    got = run(c, cuda)
+    assert torch.isinf(got).any() and not torch.isnan(got).any()
+    check(c, got)

@@ -113,7 +113,9 @@ paged_tree_kernel(const TreeParams p) {
   int* col_token = reinterpret_cast<int*>(col_scale + COLS);  // query token of a column, -1: none
   int* col_head = col_token + COLS;
 
-  // Waits for the kernel ahead (the store of this step's rows).
+  // Waits for the kernel ahead (the store of this step's rows). Global memory is read
+  // after it and by ordinary loads: the read-only path is for data that nothing writes
+  // during the kernel's lifetime, which begins while the kernel ahead still runs.
   pdl_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, c = lane & 3;
@@ -137,7 +139,7 @@ paged_tree_kernel(const TreeParams p) {
   // stage's block is read beside that length, not after it.
   int early = 0;
   if (p.cluster == 1)
-    early = __ldg(bt + min(quotient(sp * p.chunk + warp * S::kTok + lane), p.max_blocks - 1));
+    early = bt[min(quotient(sp * p.chunk + warp * S::kTok + lane), p.max_blocks - 1)];
 
   int row0 = b, n = 1;
   if (p.cu_seqlens_q) {
@@ -178,7 +180,7 @@ paged_tree_kernel(const TreeParams p) {
   auto block_of = [&](int i) {
     const int key = first_key(i) + lane;
     if (i >= mine || lane >= S::kTok || key >= key1) return -1;
-    const int blk = i == 0 && p.cluster == 1 ? early : __ldg(bt + quotient(key));
+    const int blk = i == 0 && p.cluster == 1 ? early : bt[quotient(key)];
     if (blk < 0 || blk >= p.num_blocks) {
       if (p.status) atomicOr(p.status, LK_STATUS_BLOCK_OOB);
       return -1;
@@ -313,9 +315,9 @@ paged_tree_kernel(const TreeParams p) {
         } else {
           const int64_t* row = p.mask + static_cast<int64_t>(row0 + token) * p.mask_stride;
           const int at = lo >> 6, sh = lo & 63;
-          const uint64_t a = at < p.mask_words ? static_cast<uint64_t>(__ldg(row + at)) : 0ull;
+          const uint64_t a = at < p.mask_words ? static_cast<uint64_t>(row[at]) : 0ull;
           const uint64_t n = sh > 32 && at + 1 < p.mask_words
-                                 ? static_cast<uint64_t>(__ldg(row + at + 1)) << (64 - sh)
+                                 ? static_cast<uint64_t>(row[at + 1]) << (64 - sh)
                                  : 0ull;
           w = static_cast<uint32_t>((a >> sh) | n);
         }

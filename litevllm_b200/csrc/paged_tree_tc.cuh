@@ -103,7 +103,8 @@ paged_tree_tc_kernel(const __grid_constant__ CUtensorMap kmap,
   uint8_t* sV = sK + 2 * S::kT;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-  // Set-up before the wait for the kernel ahead (the store of this step's rows).
+  // Set-up before the wait for the kernel ahead (the store of this step's rows); global
+  // memory is read after it, by ordinary loads (paged_tree.cuh says why).
   if (threadIdx.x == 0) {
     mbar_init(&q_full, 4);
     for (int i = 0; i < 2; ++i) {
@@ -173,7 +174,7 @@ paged_tree_tc_kernel(const __grid_constant__ CUtensorMap kmap,
     const int key = key0 + k0 * kChunk + lane * 16;
     if (chunks == 0 || key >= key1) return none;
     const int q = tree_quotient(p, key);
-    const int blk = __ldg(bt + q);
+    const int blk = bt[q];
     if (blk < 0 || blk >= p.num_blocks) {
       if (p.status) atomicOr(p.status, LK_STATUS_BLOCK_OOB);
       return none;
@@ -362,15 +363,14 @@ paged_tree_tc_kernel(const __grid_constant__ CUtensorMap kmap,
       float2 cur, nxt = make_float2(0.f, 0.f);
       auto block_at = [&](int k) {
         const int key = key0 + k * kChunk + g;
-        blk = k < chunks && key < key1 ? __ldg(bt + tree_quotient(p, key)) : -1;
+        blk = k < chunks && key < key1 ? bt[tree_quotient(p, key)] : -1;
         if (blk >= p.num_blocks) blk = -1;  // flagged by the copies
       };
       auto scales = [&](int k) {
         const int key = key0 + k * kChunk + g;
         const int64_t at = (static_cast<int64_t>(blk) * p.H_kv + kvh) * p.bs +
                            (key - tree_quotient(p, key) * p.bs);
-        nxt = blk < 0 ? make_float2(0.f, 0.f)
-                      : make_float2(__ldg(p.k_scale + at), __ldg(p.v_scale + at));
+        nxt = blk < 0 ? make_float2(0.f, 0.f) : make_float2(p.k_scale[at], p.v_scale[at]);
       };
       if (!is_v) {
         block_at(0);
@@ -450,8 +450,8 @@ paged_tree_tc_kernel(const __grid_constant__ CUtensorMap kmap,
     uint64_t mask_a = 0ull, mask_b = 0ull;
     const int64_t* mask = p.mask ? p.mask + qrow * p.mask_stride : nullptr;
     if (mask) {
-      if (word0 < p.mask_words) mask_a = __ldg(mask + word0);
-      if (word0 + 1 < p.mask_words) mask_b = __ldg(mask + word0 + 1);
+      if (word0 < p.mask_words) mask_a = mask[word0];
+      if (word0 + 1 < p.mask_words) mask_b = mask[word0 + 1];
     }
     float cs = p.scale_log2;
     if (warp_ok) {
@@ -467,7 +467,7 @@ paged_tree_tc_kernel(const __grid_constant__ CUtensorMap kmap,
         const int rg = tile * kRows + rr;
         const int tok = tree_token(p, rg);
         const T* src = qb + static_cast<int64_t>(row0 + tok) * p.q_stride + (rg - tok * p.G) * D;
-        if (vec) return __ldg(reinterpret_cast<const uint4*>(src));
+        if (vec) return *reinterpret_cast<const uint4*>(src);
         const uint16_t* s = reinterpret_cast<const uint16_t*>(src);
         return make_uint4(s[0] | (s[1] << 16), s[2] | (s[3] << 16), s[4] | (s[5] << 16),
                           s[6] | (s[7] << 16));
@@ -530,8 +530,8 @@ paged_tree_tc_kernel(const __grid_constant__ CUtensorMap kmap,
           const int at = lo >> 6, sh = lo & 63;
           uint64_t a = mask_a, c = mask_b;
           if (at != word0) {
-            a = at < p.mask_words ? static_cast<uint64_t>(__ldg(mask + at)) : 0ull;
-            c = at + 1 < p.mask_words ? static_cast<uint64_t>(__ldg(mask + at + 1)) : 0ull;
+            a = at < p.mask_words ? static_cast<uint64_t>(mask[at]) : 0ull;
+            c = at + 1 < p.mask_words ? static_cast<uint64_t>(mask[at + 1]) : 0ull;
           }
           w = a >> sh;
           if (sh) w |= c << (64 - sh);

@@ -70,3 +70,34 @@ def test_special_values_beside_rows_that_fill_no_warp(cuda, dtype):
     got = run(c, cuda)
     assert torch.isinf(got).any() and not torch.isnan(got).any()
     check(c, got)
+
+
+@pytest.mark.parametrize("kind", [INT8, E4M3])
+def test_rows_and_scales_stored_right_before_are_read(cuda, kind):
+    """Steps of store, tree attention, store, ... with no wait between them, each of rows of
+    another size in the same slots, give what the same steps give one at a time."""
+    from litevllm_b200 import ops
+    from tests.spec_inputs import on, randn
+
+    c = late_maxima(kind, [9, 13, 11, 13] * 3, seed=7)
+    k, v = on(cuda, c["kd"], c["ks"]), on(cuda, c["vd"], c["vs"])
+    slots = []
+    for b, (n, ctx) in enumerate(zip(c["counts"], c["ctx"])):
+        slots += [c["tables"][b, p // 16].item() * 16 + p % 16 for p in range(ctx - n, ctx)]
+    slots = torch.tensor(slots, device=cuda)
+    rows = [randn(i, len(slots), 8, 128, dtype=BF16, std=2.0 ** (3 * (i % 4) - 6)).to(cuda) for i in range(8)]
+    args = (c["q"].to(cuda), k, v, c["tables"].to(cuda), torch.tensor(c["ctx"], dtype=torch.int32).to(cuda),
+            c["cu"].to(cuda), max(c["counts"]), c["scale"])
+    mask = c["mask"].to(cuda)
+
+    def step(i, wait):
+        ops.store_kvcache_q8(rows[i], rows[(i + 3) % 8], k, v, slots)
+        if wait:
+            torch.cuda.synchronize()
+        return ops.paged_tree_attention(*args, tree_mask=mask)
+
+    want = [step(i, True) for i in range(8)]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        got = [step(i, False) for i in range(8)]
+        assert all(torch.equal(a, b) for a, b in zip(got, want))

@@ -604,11 +604,11 @@ paged_tree_tc_kernel(const __grid_constant__ CUtensorMap kmap,
               tc::wait_st();
             }
           }
+          __syncwarp();  // inside weigh() it costs 84 bytes of spills
           float top = -INFINITY;  // of the exponents (8-bit: of the weights)
           sum0 = sum1 = 0.f;
           auto weigh = [&](auto with_mask) {
             uint32_t sv[64];
-            __syncwarp();
             tc::ld32(tS, *reinterpret_cast<uint32_t(*)[32]>(sv));
             tc::ld32(tS + 32, *reinterpret_cast<uint32_t(*)[32]>(sv + 32));
             tc::wait_ld();

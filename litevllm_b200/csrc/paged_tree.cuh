@@ -141,15 +141,8 @@ paged_tree_kernel(const TreeParams p) {
   if (p.cluster == 1)
     early = bt[min(quotient(sp * p.chunk + warp * S::kTok + lane), p.max_blocks - 1)];
 
-  int row0 = b, n = 1;
-  if (p.cu_seqlens_q) {
-    row0 = p.cu_seqlens_q[b];
-    n = p.cu_seqlens_q[b + 1] - row0;
-    if (n > p.max_q || row0 < 0 || row0 + n > p.T) {  // a bad cu_seqlens_q: nothing outside q
-      if (threadIdx.x == 0 && p.status) atomicOr(p.status, LK_STATUS_CTX_OOB);
-      n = row0 < 0 ? 0 : min(min(n, p.max_q), p.T - row0);
-    }
-  }
+  int row0;
+  const int n = tree_tokens(p, b, &row0);
   const int rows = n * p.G;  // query rows of this KV head
   if (cg * COLS >= rows) return;
   int ctx = p.context_lens[b];

@@ -41,6 +41,21 @@ struct TreeParams {
 };
 
 #ifdef __CUDACC__
+// Query tokens of sequence b, rows row0 .. of q. A cu_seqlens_q that passes q or max_q is
+// flagged and cut to what lies inside both. In 64 bits: the difference of two entries and
+// the end of the rows may pass 32.
+__device__ __forceinline__ int tree_tokens(const TreeParams& p, int b, int* row0) {
+  *row0 = b;
+  if (!p.cu_seqlens_q) return 1;
+  const int64_t first = p.cu_seqlens_q[b];
+  const int64_t count = p.cu_seqlens_q[b + 1] - first;
+  *row0 = static_cast<int>(first);
+  if (count <= p.max_q && first >= 0 && first + count <= p.T)
+    return static_cast<int>(max(count, static_cast<int64_t>(0)));
+  if (threadIdx.x == 0 && p.status) atomicOr(p.status, LK_STATUS_CTX_OOB);
+  if (first < 0 || first >= p.T || count <= 0) return 0;
+  return static_cast<int>(min(min(count, static_cast<int64_t>(p.max_q)), p.T - first));
+}
 // key / p.bs, key < 2^31.
 __device__ __forceinline__ int tree_quotient(const TreeParams& p, int key) {
   return static_cast<int>(p.bs_mul ? __umulhi(key, p.bs_mul) >> p.bs_shift

@@ -142,12 +142,8 @@ paged_tree_tc_kernel(const __grid_constant__ CUtensorMap kmap,
   rest /= p.H_kv;
   const int b = rest % p.B;
   const int sp = rest / p.B;
-  const int row0 = p.cu_seqlens_q ? p.cu_seqlens_q[b] : b;
-  int n = p.cu_seqlens_q ? p.cu_seqlens_q[b + 1] - row0 : 1;
-  if (n > p.max_q || row0 < 0 || row0 + n > p.T) {
-    if (threadIdx.x == 0 && p.status) atomicOr(p.status, LK_STATUS_CTX_OOB);
-    n = row0 < 0 ? 0 : min(min(n, p.max_q), p.T - row0);
-  }
+  int row0;
+  const int n = tree_tokens(p, b, &row0);
   int ctx = p.context_lens[b];
   if (ctx > p.max_blocks * p.bs || ctx < (p.cu_seqlens_q ? n : 0)) {
     if (threadIdx.x == 0 && p.status) atomicOr(p.status, LK_STATUS_CTX_OOB);

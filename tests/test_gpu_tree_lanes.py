@@ -7,6 +7,7 @@ import random
 import pytest
 import torch
 
+from litevllm_b200 import _lib
 from oracle import kv_q8
 from tests.test_gpu_tree import BF16, E4M3, F16, INT8, case, check, run
 
@@ -101,3 +102,22 @@ def test_rows_and_scales_stored_right_before_are_read(cuda, kind):
     for _ in range(20):
         got = [step(i, False) for i in range(8)]
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("width", [None, 256], ids=["few rows", "many rows"])
+@pytest.mark.parametrize("ends", [(2 ** 31 - 8, -2 ** 31), (2 ** 31 - 1, 2 ** 31 - 1), (-2 ** 31, 5),
+                                  (2 ** 31 - 8, 2 ** 31 - 4)])
+def test_sequence_bounds_that_pass_32_bits(cuda, width, ends):
+    """Entries of cu_seqlens_q whose difference, or whose rows' end, does not fit 32
+    bits: flagged, the first sequence's rows up to max_q_len computed, no other touched."""
+    counts = [13] + [9] * 11
+    c = late_maxima(BF16, counts, seed=9) if width else case(BF16, BF16, 8, 2, 128, 16, [250] * 12, counts, seed=9)
+    good = run(c, cuda)
+    c["cu"] = torch.tensor([0, *ends] + [0] * 10, dtype=torch.int32)
+    out = torch.full_like(good, 5.0)
+    status = torch.zeros(1, dtype=torch.int32, device=cuda)
+    run(c, cuda, out=out, status=status)
+    torch.cuda.synchronize()
+    assert status.item() & _lib.LK_STATUS_CTX_OOB
+    rows = 13 if ends[0] > 0 else 0
+    assert torch.equal(out[:rows], good[:rows]) and (out[rows:] == 5).all()

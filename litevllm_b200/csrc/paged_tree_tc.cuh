@@ -651,7 +651,9 @@ paged_tree_tc_kernel(const __grid_constant__ CUtensorMap kmap,
           if (masked) weigh(std::true_type());
           else weigh(std::false_type());
           if (raise) break;
-          up = top > (S::kQ8 ? 256.f : kRaise);
+          // 8-bit: a weight is small, or 0 times infinity, where s_v is, while its 2^(x - M)
+          // in the denominator passes all bounds; raised maxima keep the sum below 2^106
+          up = S::kQ8 ? top > 256.f || sum0 + sum1 > 0x1p110f : top > kRaise;
           raise = __any_sync(0xffffffffu, up);
           if (!raise) break;
         }

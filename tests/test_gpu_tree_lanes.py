@@ -121,3 +121,24 @@ def test_sequence_bounds_that_pass_32_bits(cuda, width, ends):
     assert status.item() & _lib.LK_STATUS_CTX_OOB
     rows = 13 if ends[0] > 0 else 0
     assert torch.equal(out[:rows], good[:rows]) and (out[rows:] == 5).all()
+
+
+@pytest.mark.parametrize("kind", [INT8, E4M3])
+@pytest.mark.parametrize("counts", [[9, 13, 11, 13] * 3, [3, 2, 4] * 4], ids=["many rows", "few rows"])
+def test_rows_of_scale_zero_outweigh_far_smaller_scores(cuda, kind, counts):
+    """A slot that was never written (scale 0: its key scores 0, its value is 0) behind
+    keys whose scores are about -120: it takes all the weight, and the result is 0."""
+    c = late_maxima(kind, counts, seed=3)
+    c["q"] = c["q"][:1, :1].expand_as(c["q"]).contiguous()
+    q = c["q"][0, 0].float()
+    rows = (-120.0 * q / q.norm()).expand(8, 128) * (128 ** 0.5 / q.norm())
+    for b, ctx in enumerate(c["ctx"]):
+        for p in range(ctx):
+            put_row(c, "k", b, p, rows)
+        blk, off = c["tables"][b, 100 // 16], 100 % 16
+        for x in "kv":
+            c[x + "d"].view(torch.uint8)[blk, off] = 0
+            c[x + "s"][blk, :, off] = 0.0
+    got = run(c, cuda)
+    check(c, got)
+    assert (got == 0).all()

@@ -94,10 +94,9 @@ def _prefill(query, key_cache, value_cache, cu_seqlens_q, max_q_len, scale, bloc
     uses each key many times, the copy moves it twice."""
     if isinstance(key_cache, ops.QuantizedCache):
         nb, bs, H_kv, D = key_cache.data.shape
-        S, blocks = block_tables.shape
+        S, blocks = block_tables.shape[0], max(1, block_tables.shape[1])
         dev = query.device
-        cu_rows = torch.arange(0, S * blocks * bs + 1, max(1, blocks * bs), dtype=torch.int32,
-                               device=dev)
+        cu_rows = torch.arange(0, S * blocks * bs + 1, blocks * bs, dtype=torch.int32, device=dev)
         key_cache, value_cache = (
             x.view(S * blocks, bs, H_kv, D) for x in ops.load_kvcache_q8(
                 key_cache, value_cache, block_tables, context_lens, cu_rows, S * blocks * bs,

@@ -124,6 +124,22 @@ int lk_load_kv_q8(void* key_out, void* value_out, const void* k_data, const floa
                   int32_t* status, void* stream);
 
 /*
+ * Read the contexts of an 8-bit cache back as whole blocks, for kernels that read
+ * 16- or 32-bit caches: block i of sequence b becomes block
+ * n = b * max_blocks_per_seq + i of key_out / value_out ([num_seqs *
+ * max_blocks_per_seq, block_size, H_kv, D]) where it holds a token of the
+ * context, with zeros behind the last one; other blocks are left as they were.
+ * out_tables [num_seqs, max_blocks_per_seq]: n, for every i. Types, roundings
+ * and flags as for lk_load_kv_q8.
+ */
+int lk_load_kv_q8_blocks(void* key_out, void* value_out, int32_t* out_tables, const void* k_data,
+                         const float* k_scale, const void* v_data, const float* v_scale,
+                         const int32_t* block_tables, int64_t block_table_stride,
+                         const int32_t* context_lens, int32_t num_seqs, int32_t H_kv, int32_t D,
+                         int64_t num_blocks, int32_t block_size, int32_t max_blocks_per_seq,
+                         int32_t dtype, int32_t kv_format, int32_t* status, void* stream);
+
+/*
  * Paged decode attention. Replaces Attention._decode_fast,
  * litevllm/layers/attention.py:91-139:
  *   out[b,h,:] = softmax_s(scale * q[b,h] . k[b,s,h/G]) @ v[b,s,h/G],

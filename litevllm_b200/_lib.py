@@ -45,6 +45,12 @@ SIGNATURES: dict[str, tuple] = {
          c_void_p, c_int32, c_int64, c_int32, c_int32, c_int64, c_int32, c_int32, c_int32,
          c_int32, c_void_p, c_void_p],
     ),
+    "lk_load_kv_q8_blocks": (
+        c_int32,
+        [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64,
+         c_void_p, c_int32, c_int32, c_int32, c_int64, c_int32, c_int32, c_int32, c_int32,
+         c_void_p, c_void_p],
+    ),
     "lk_paged_decode_num_splits": (c_int32, [c_int32, c_int32, c_int32, c_int32]),
     "lk_paged_decode_workspace_bytes": (c_size_t, [c_int32, c_int32, c_int32, c_int32, c_int32]),
     "lk_paged_decode": (

@@ -63,12 +63,13 @@ _MIXED_STEP = {"table": None}
 
 def set_mixed_step_hint(block_tables: Optional[torch.Tensor], cu_seqlens_q=None,
                         num_prefill_seqs: int = 0, num_prefill_tokens: int = 0,
-                        max_q_len: int = 0) -> None:
+                        max_q_len: int = 0, max_prefill_blocks: Optional[int] = None) -> None:
     """Declare the mixed layout of the step whose table is `block_tables`
     (None clears the hint)."""
     _MIXED_STEP.clear()
     _MIXED_STEP.update(table=block_tables, cu_seqlens_q=cu_seqlens_q, P=int(num_prefill_seqs),
-                       TP=int(num_prefill_tokens), max_q_len=int(max_q_len))
+                       TP=int(num_prefill_tokens), max_q_len=int(max_q_len),
+                       max_prefill_blocks=max_prefill_blocks)
 
 
 def set_shared_prefix_hint(block_tables: Optional[torch.Tensor], prefix_tokens: int) -> None:
@@ -86,24 +87,41 @@ def _store(key, value, key_cache, value_cache, slot_mapping) -> None:
         ops.store_kvcache(key, value, key_cache, value_cache, slot_mapping)
 
 
+# Most bytes of 16-bit blocks that prefill over an 8-bit cache holds at a time, where one
+# sequence's table does not take more: above, sequences are read back and attended some
+# at a time. A GB is two tables of 128K tokens, or 32 of 8K, with 8 KV heads of 128.
+Q8_PREFILL_BYTES = 1 << 30
+
+
 def _prefill(query, key_cache, value_cache, cu_seqlens_q, max_q_len, scale, block_tables,
              context_lens, out=None) -> torch.Tensor:
     """paged_prefill over 16-bit caches or a QuantizedCache pair. The 8-bit
-    contexts are read back once into 16-bit blocks of this call's own, every
-    sequence's in order, which the prefill kernel then reads: a chunk of queries
-    uses each key many times, the copy moves it twice."""
-    if isinstance(key_cache, ops.QuantizedCache):
-        nb, bs, H_kv, D = key_cache.data.shape
-        S, blocks = block_tables.shape[0], max(1, block_tables.shape[1])
-        dev = query.device
-        cu_rows = torch.arange(0, S * blocks * bs + 1, blocks * bs, dtype=torch.int32, device=dev)
-        key_cache, value_cache = (
-            x.view(S * blocks, bs, H_kv, D) for x in ops.load_kvcache_q8(
-                key_cache, value_cache, block_tables, context_lens, cu_rows, S * blocks * bs,
-                dtype=query.dtype))
-        block_tables = torch.arange(S * blocks, dtype=torch.int32, device=dev).view(S, blocks)
-    return ops.paged_prefill(query, key_cache, value_cache, cu_seqlens_q, max_q_len, scale,
-                             block_tables=block_tables, context_lens=context_lens, out=out)
+    contexts are read back once into 16-bit blocks of this call's own, which the
+    prefill kernel then reads: a chunk of queries uses each key many times, the copy
+    moves it twice. The blocks are allotted by the table's width (the contexts are on
+    the device) and written as far as the contexts go. Their rows are rounded to the
+    query's type, the prefill kernel's operand; decode and tree attention read them
+    exactly."""
+    if not isinstance(key_cache, ops.QuantizedCache):
+        return ops.paged_prefill(query, key_cache, value_cache, cu_seqlens_q, max_q_len, scale,
+                                 block_tables=block_tables, context_lens=context_lens, out=out)
+    if out is None:
+        out = torch.empty(query.shape, dtype=query.dtype, device=query.device)
+    S, blocks = block_tables.shape
+    if S == 0 or query.shape[0] == 0:
+        return out
+    if blocks == 0:
+        raise ValueError("block_tables has no columns for the new tokens")
+    each = 2 * blocks * key_cache.data[0].numel() * query.element_size()
+    step = max(1, Q8_PREFILL_BYTES // each)
+    for b in range(0, S, step):
+        some = slice(b, b + step)
+        k, v, tables = ops.load_kvcache_q8_blocks(key_cache, value_cache, block_tables[some],
+                                                  context_lens[some], dtype=query.dtype)
+        ops.paged_prefill(query, k, v, cu_seqlens_q[b:b + step + 1], max_q_len, scale,
+                          block_tables=tables, context_lens=context_lens[some], out=out)
+        del k, v, tables  # before the next ones are allotted
+    return out
 
 
 def _decode(query, key_cache, value_cache, block_tables, context_lens, scale, out=None):
@@ -180,7 +198,8 @@ class Attention(nn.Module):
             # a merged prefill + decode step (engine_hooks.prepare_inputs_mixed)
             return self.forward_mixed(
                 query, key, value, key_cache, value_cache, block_table, slot_mapping,
-                context_lens, mixed["cu_seqlens_q"], mixed["P"], mixed["TP"], mixed["max_q_len"])
+                context_lens, mixed["cu_seqlens_q"], mixed["P"], mixed["TP"], mixed["max_q_len"],
+                mixed["max_prefill_blocks"])
 
         if slot_mapping is not None and key_cache is not None:
             _store(key, value, key_cache, value_cache, slot_mapping)
@@ -261,6 +280,7 @@ class Attention(nn.Module):
         num_prefill_seqs: int,
         num_prefill_tokens: int,
         max_q_len: int,
+        max_prefill_blocks: Optional[int] = None,
     ) -> torch.Tensor:
         """One mixed chunked-prefill + decode step.
 
@@ -269,7 +289,9 @@ class Attention(nn.Module):
         remaining rows are one decode token per sequence. All K/V are stored
         first; then the prefill kernel runs on the caller's stream and the
         decode kernel on a side stream next to it (run_overlapped), joined
-        before returning.
+        before returning. max_prefill_blocks: the most blocks that a prefill
+        sequence's context takes, where the caller knows it; over an 8-bit cache
+        the space for their contexts goes by it instead of the table's width.
         """
         if slot_mapping is not None:
             _store(key, value, key_cache, value_cache, slot_mapping)
@@ -279,7 +301,7 @@ class Attention(nn.Module):
         def prefill():
             _prefill(
                 query[:TP], key_cache, value_cache, cu_seqlens_q[: P + 1], max_q_len, self.scale,
-                block_tables=block_table[:P], context_lens=context_lens[:P], out=out[:TP],
+                block_tables=block_table[:P, :max_prefill_blocks], context_lens=context_lens[:P], out=out[:TP],
             )
 
         def decode():

@@ -126,6 +126,7 @@ struct LoadQ8Params {
   int64_t bt_stride;
   const int32_t* context_lens;
   const int32_t* cu_rows;     // [B + 1]
+  int32_t* out_tables;        // [B, max_blocks], instead of cu_rows: whole blocks
   int64_t num_blocks;
   int64_t num_rows;
   int B, H_kv, bs, max_blocks;
@@ -147,34 +148,47 @@ template <> LK_DEVINL void put8<float>(float* dst, const float (&x)[8]) {
 // contiguous over the warp), up to eight loads under way at once. K and V one after
 // the other took 82 us instead of 68 for 69K rows of 8 x 128; two rows a warp, to
 // share the search, 70, four 71 (and short calls lose warps: 6.2K rows 7.8, 8.0, 10).
-template <typename T, int FMT, int D>
+// BLOCKS: the output is blocks in the table's order, of which those with a token of the
+// context are written (zeros behind it); a row that is not costs its warp's start.
+template <typename T, int FMT, int D, bool BLOCKS>
 __global__ void __launch_bounds__(kQThreads) load_kv_q8_kernel(const LoadQ8Params p) {
   const int lane = threadIdx.x & 31;
   const int64_t at = static_cast<int64_t>(blockIdx.x) * (kQThreads / 32) + (threadIdx.x >> 5);
-  if (at >= p.num_rows || at < p.cu_rows[0] || at >= p.cu_rows[p.B]) return;
+  if (at >= p.num_rows || (!BLOCKS && (at < p.cu_rows[0] || at >= p.cu_rows[p.B]))) return;
   const int row = static_cast<int>(at);
-  // b = the last sequence that starts at or before row: 32 probes a step
-  int lo = 0, hi = p.B;  // cu_rows[lo] <= row < cu_rows[hi]
-  while (hi - lo > 1) {
-    const int step = (hi - lo + 31) / 32;
-    const int probe = min(lo + lane * step, hi);
-    const uint32_t le = __ballot_sync(0xffffffffu, p.cu_rows[probe] <= row);
-    const int k = 31 - __clz(le);  // lane 0 always holds
-    const int nlo = min(lo + k * step, hi - 1);
-    hi = min(hi, nlo + step);
-    lo = nlo;
+  int b, pos;
+  if constexpr (BLOCKS) {
+    const uint32_t cap = p.max_blocks * p.bs;
+    b = static_cast<uint32_t>(row) / cap;
+    pos = row - b * cap;
+  } else {
+    // b = the last sequence that starts at or before row: 32 probes a step
+    int lo = 0, hi = p.B;  // cu_rows[lo] <= row < cu_rows[hi]
+    while (hi - lo > 1) {
+      const int step = (hi - lo + 31) / 32;
+      const int probe = min(lo + lane * step, hi);
+      const uint32_t le = __ballot_sync(0xffffffffu, p.cu_rows[probe] <= row);
+      const int k = 31 - __clz(le);  // lane 0 always holds
+      const int nlo = min(lo + k * step, hi - 1);
+      hi = min(hi, nlo + step);
+      lo = nlo;
+    }
+    b = lo;
+    pos = row - p.cu_rows[b];
   }
-  const int b = lo;
-  const int pos = row - p.cu_rows[b];
   int ctx = p.context_lens[b];
   if (ctx > p.max_blocks * static_cast<int64_t>(p.bs)) {
     if (lane == 0 && p.status) atomicOr(p.status, LK_STATUS_CTX_OOB);
     ctx = p.max_blocks * p.bs;
   }
-  int blk = -1, off = 0;
+  const int page = static_cast<uint32_t>(max(pos, 0)) / static_cast<uint32_t>(p.bs);
+  const int off = pos - page * p.bs;
+  if constexpr (BLOCKS) {
+    if (off == 0 && lane == 0) p.out_tables[row / p.bs] = row / p.bs;
+    if (page * p.bs >= ctx) return;
+  }
+  int blk = -1;
   if (pos >= 0 && pos < ctx) {
-    const int page = static_cast<uint32_t>(pos) / static_cast<uint32_t>(p.bs);
-    off = pos - page * p.bs;
     blk = p.block_tables[b * p.bt_stride + page];
     if (blk < 0 || blk >= p.num_blocks) {
       if (lane == 0 && p.status) atomicOr(p.status, LK_STATUS_BLOCK_OOB);
@@ -240,6 +254,65 @@ bool kv_q8_shape(int32_t H_kv, int32_t D, int32_t bs, int64_t num_blocks, int32_
 
 bool aligned16(const void* a) { return (reinterpret_cast<uintptr_t>(a) & 15u) == 0; }
 
+// Shared by the two entry points: cu_rows or out_tables is NULL.
+int load_kv_q8(void* key_out, void* value_out, const void* k_data, const float* k_scale,
+               const void* v_data, const float* v_scale, const int32_t* block_tables,
+               int64_t block_table_stride, const int32_t* context_lens, const int32_t* cu_rows,
+               int32_t* out_tables, int32_t num_seqs, int64_t num_rows, int32_t H_kv, int32_t D,
+               int64_t num_blocks, int32_t block_size, int32_t max_blocks_per_seq, int32_t dtype,
+               int32_t kv_format, int32_t* status, void* stream) {
+  int rc = LK_OK;
+  if (num_seqs < 0 || num_rows < 0 || max_blocks_per_seq < 0) return LK_ERR_INVALID_ARG;
+  if (!kv_q8_shape(H_kv, D, block_size, num_blocks, kv_format, &rc)) return rc;
+  if (dtype != LK_DTYPE_F32 && dtype != LK_DTYPE_F16 && dtype != LK_DTYPE_BF16)
+    return LK_ERR_UNSUPPORTED;
+  if (num_seqs == 0 || num_rows == 0) return LK_OK;
+  if (!key_out || !value_out || !k_data || !k_scale || !v_data || !v_scale || !context_lens ||
+      (!cu_rows && !out_tables) || (max_blocks_per_seq > 0 && !block_tables) ||
+      num_rows > 0x7fffffffLL || max_blocks_per_seq > 0x7fffffff / block_size)
+    return LK_ERR_INVALID_ARG;
+  if (!aligned16(k_data) || !aligned16(v_data) || !aligned16(key_out) || !aligned16(value_out))
+    return LK_ERR_ALIGNMENT;
+  LoadQ8Params p;
+  p.data[0] = static_cast<const uint8_t*>(k_data);
+  p.data[1] = static_cast<const uint8_t*>(v_data);
+  p.scale[0] = k_scale;
+  p.scale[1] = v_scale;
+  p.out[0] = key_out;
+  p.out[1] = value_out;
+  p.block_tables = block_tables;
+  p.bt_stride = block_table_stride;
+  p.context_lens = context_lens;
+  p.cu_rows = cu_rows;
+  p.out_tables = out_tables;
+  p.num_blocks = num_blocks;
+  p.num_rows = num_rows;
+  p.B = num_seqs;
+  p.H_kv = H_kv;
+  p.bs = block_size;
+  p.max_blocks = max_blocks_per_seq;
+  p.status = status;
+  const int per_cta = kQThreads / 32;
+  const unsigned grid = static_cast<unsigned>((num_rows + per_cta - 1) / per_cta);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  auto by_dim = [&](auto type, auto fmt) {
+    using T = decltype(type);
+    constexpr int F = decltype(fmt)::value;
+    if (out_tables && D == 128) load_kv_q8_kernel<T, F, 128, true><<<grid, kQThreads, 0, s>>>(p);
+    else if (out_tables) load_kv_q8_kernel<T, F, 64, true><<<grid, kQThreads, 0, s>>>(p);
+    else if (D == 128) load_kv_q8_kernel<T, F, 128, false><<<grid, kQThreads, 0, s>>>(p);
+    else load_kv_q8_kernel<T, F, 64, false><<<grid, kQThreads, 0, s>>>(p);
+  };
+  auto by_fmt = [&](auto type) {
+    if (kv_format == LK_KV_INT8) by_dim(type, std::integral_constant<int, LK_KV_INT8>());
+    else by_dim(type, std::integral_constant<int, LK_KV_E4M3>());
+  };
+  if (dtype == LK_DTYPE_BF16) by_fmt(__nv_bfloat16());
+  else if (dtype == LK_DTYPE_F16) by_fmt(__half());
+  else by_fmt(float());
+  return lk::check_launch();
+}
+
 }  // namespace
 
 extern "C" int lk_store_kv_q8(const void* key, const void* value, void* k_data, float* k_scale,
@@ -303,51 +376,24 @@ extern "C" int lk_load_kv_q8(void* key_out, void* value_out, const void* k_data,
                              int32_t num_seqs, int64_t num_rows, int32_t H_kv, int32_t D,
                              int64_t num_blocks, int32_t block_size, int32_t max_blocks_per_seq,
                              int32_t dtype, int32_t kv_format, int32_t* status, void* stream) {
-  int rc = LK_OK;
-  if (num_seqs < 0 || num_rows < 0 || max_blocks_per_seq < 0) return LK_ERR_INVALID_ARG;
-  if (!kv_q8_shape(H_kv, D, block_size, num_blocks, kv_format, &rc)) return rc;
-  if (dtype != LK_DTYPE_F32 && dtype != LK_DTYPE_F16 && dtype != LK_DTYPE_BF16)
-    return LK_ERR_UNSUPPORTED;
-  if (num_seqs == 0 || num_rows == 0) return LK_OK;
-  if (!key_out || !value_out || !k_data || !k_scale || !v_data || !v_scale || !context_lens ||
-      !cu_rows || (max_blocks_per_seq > 0 && !block_tables) || num_rows > 0x7fffffffLL ||
-      max_blocks_per_seq > 0x7fffffff / block_size)
-    return LK_ERR_INVALID_ARG;
-  if (!aligned16(k_data) || !aligned16(v_data) || !aligned16(key_out) || !aligned16(value_out))
-    return LK_ERR_ALIGNMENT;
-  LoadQ8Params p;
-  p.data[0] = static_cast<const uint8_t*>(k_data);
-  p.data[1] = static_cast<const uint8_t*>(v_data);
-  p.scale[0] = k_scale;
-  p.scale[1] = v_scale;
-  p.out[0] = key_out;
-  p.out[1] = value_out;
-  p.block_tables = block_tables;
-  p.bt_stride = block_table_stride;
-  p.context_lens = context_lens;
-  p.cu_rows = cu_rows;
-  p.num_blocks = num_blocks;
-  p.num_rows = num_rows;
-  p.B = num_seqs;
-  p.H_kv = H_kv;
-  p.bs = block_size;
-  p.max_blocks = max_blocks_per_seq;
-  p.status = status;
-  const int per_cta = kQThreads / 32;
-  const unsigned grid = static_cast<unsigned>((num_rows + per_cta - 1) / per_cta);
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
-  auto by_dim = [&](auto type, auto fmt) {
-    using T = decltype(type);
-    constexpr int F = decltype(fmt)::value;
-    if (D == 128) load_kv_q8_kernel<T, F, 128><<<grid, kQThreads, 0, s>>>(p);
-    else load_kv_q8_kernel<T, F, 64><<<grid, kQThreads, 0, s>>>(p);
-  };
-  auto by_fmt = [&](auto type) {
-    if (kv_format == LK_KV_INT8) by_dim(type, std::integral_constant<int, LK_KV_INT8>());
-    else by_dim(type, std::integral_constant<int, LK_KV_E4M3>());
-  };
-  if (dtype == LK_DTYPE_BF16) by_fmt(__nv_bfloat16());
-  else if (dtype == LK_DTYPE_F16) by_fmt(__half());
-  else by_fmt(float());
-  return lk::check_launch();
+  return load_kv_q8(key_out, value_out, k_data, k_scale, v_data, v_scale, block_tables,
+                    block_table_stride, context_lens, cu_rows, nullptr, num_seqs, num_rows, H_kv, D,
+                    num_blocks, block_size, max_blocks_per_seq, dtype, kv_format, status, stream);
+}
+
+extern "C" int lk_load_kv_q8_blocks(void* key_out, void* value_out, int32_t* out_tables,
+                                    const void* k_data, const float* k_scale, const void* v_data,
+                                    const float* v_scale, const int32_t* block_tables,
+                                    int64_t block_table_stride, const int32_t* context_lens,
+                                    int32_t num_seqs, int32_t H_kv, int32_t D, int64_t num_blocks,
+                                    int32_t block_size, int32_t max_blocks_per_seq, int32_t dtype,
+                                    int32_t kv_format, int32_t* status, void* stream) {
+  if (num_seqs > 0 && max_blocks_per_seq > 0 && !out_tables) return LK_ERR_INVALID_ARG;
+  if (num_seqs < 0 || max_blocks_per_seq < 0 || block_size <= 0) return LK_ERR_INVALID_ARG;
+  const int64_t blocks = static_cast<int64_t>(num_seqs) * max_blocks_per_seq;
+  if (blocks > 0x7fffffffLL / block_size) return LK_ERR_INVALID_ARG;
+  return load_kv_q8(key_out, value_out, k_data, k_scale, v_data, v_scale, block_tables,
+                    block_table_stride, context_lens, nullptr, out_tables, num_seqs,
+                    blocks * block_size, H_kv, D, num_blocks, block_size, max_blocks_per_seq, dtype,
+                    kv_format, status, stream);
 }

@@ -245,6 +245,40 @@ PyObject* load(PyObject*, PyObject* const* a, Py_ssize_t) {
   });
 }
 
+// load_blocks(key_cache, value_cache, block_tables, context_lens, dtype, status)
+PyObject* load_blocks(PyObject*, PyObject* const* a, Py_ssize_t) {
+  return guarded([&]() -> PyObject* {
+    const Caches c = caches(a[0], a[1], false);
+    T bt = tensor(a[2]), ctx = tensor(a[3]);
+    const T status = tensor(a[5], true);
+    const int dev = device_of({c.kd, c.ks, c.vd, c.vs, bt, ctx, status});
+    if (bt->scalar_type() != at::kInt || bt->dim() != 2) type_error("block_tables must be int32 [B, max_blocks]");
+    const int64_t B = bt->size(0), max_blocks = bt->size(1);
+    at::Tensor bt_keep, ctx_keep;
+    if (max_blocks > 0 && bt->stride(1) != 1) {
+      bt_keep = bt->contiguous();
+      bt = &bt_keep;
+    }
+    ctx = int32_row(ctx, B, "context_lens must be int32 [B]", ctx_keep);
+    check_status(status);
+    if (!THPDtype_Check(a[4])) type_error("dtype must be a torch.dtype");
+    const at::ScalarType type = reinterpret_cast<THPDtype*>(a[4])->scalar_type;
+    const int code = dtype_code(type, true);
+    const c10::cuda::CUDAGuard guard(dev);
+    const at::Tensor outs[3] = {at::empty({B * max_blocks, c.bs, c.H_kv, c.D}, c.kd->options().dtype(type)),
+                                at::empty({B * max_blocks, c.bs, c.H_kv, c.D}, c.kd->options().dtype(type)),
+                                at::empty({B, max_blocks}, c.kd->options().dtype(at::kInt))};
+    call(lk_load_kv_q8_blocks, outs[0].data_ptr(), outs[1].data_ptr(), ptr<int32_t>(&outs[2]), ptr(c.kd),
+         ptr<float>(c.ks), ptr(c.vd), ptr<float>(c.vs), ptr<int32_t>(bt), bt->stride(0), ptr<int32_t>(ctx),
+         n32(B), n32(c.H_kv), n32(c.D), c.nb, n32(c.bs), n32(max_blocks), code, c.fmt,
+         ptr<int32_t>(status), stream_of(dev));
+    PyObject* t = PyTuple_New(3);
+    if (!t) throw PyRaised();
+    for (int i = 0; i < 3; ++i) PyTuple_SET_ITEM(t, i, THPVariable_Wrap(outs[i]));
+    return t;
+  });
+}
+
 // tree(query, key_cache, value_cache, block_tables, context_lens, cu_seqlens_q, max_q_len, scale,
 //      tree_mask, out, workspace, status); max_q_len None: decode over an 8-bit cache
 PyObject* tree(PyObject*, PyObject* const* a, Py_ssize_t) {
@@ -435,8 +469,8 @@ PyMethodDef method(const char* name) {
 }
 
 PyMethodDef g_methods[] = {method<init, 2>("init"),   method<store, 6>("store"), method<load, 10>("load"),
-                           method<tree, 12>("tree"),  method<logits, 13>("logits"),
-                           {nullptr, nullptr, 0, nullptr}};
+                           method<load_blocks, 6>("load_blocks"), method<tree, 12>("tree"),
+                           method<logits, 13>("logits"), {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_spec", nullptr, -1, g_methods};
 

@@ -194,7 +194,8 @@ def prepare_inputs_mixed(self, prefill_groups, decode_groups, block_manager):
     context_lens = d32[nb:nb + len(tables)]
     cu_seqlens_q = d32[nb + len(tables):]
     set_shared_prefix_hint(None, 0)
-    set_mixed_step_hint(block_tables, cu_seqlens_q, P, int(cu[-1]), max(q_lens))
+    set_mixed_step_hint(block_tables, cu_seqlens_q, P, int(cu[-1]), max(q_lens),
+                        max(max(t.shape[0] for t in tables[:P]), -(-max(ctx_lens[:P]) // bs)))
     return InputMetadata(input_ids=input_ids, positions=positions, slot_mapping=slot_mapping,
                          block_tables=block_tables, context_lens=context_lens,
                          is_prefill=True, seq_ids=seq_ids)

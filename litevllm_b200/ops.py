@@ -205,6 +205,21 @@ def load_kvcache_q8(
                         key_out, value_out, status)
 
 
+def load_kvcache_q8_blocks(
+    key_cache: QuantizedCache,
+    value_cache: QuantizedCache,
+    block_tables: torch.Tensor,
+    context_lens: torch.Tensor,
+    dtype: torch.dtype = torch.bfloat16,
+    status: Optional[torch.Tensor] = None,
+) -> tuple:
+    """The contexts of 8-bit caches as blocks of `dtype` (fp32, fp16 or bf16), for
+    kernels that read such caches: (key_cache, value_cache [B * max_blocks,
+    block_size, H_kv, D], block_tables [B, max_blocks]). Blocks that hold a token
+    of a context are written, with zeros behind it; the others hold anything."""
+    return _spec().load_blocks(key_cache, value_cache, block_tables, context_lens, dtype, status)
+
+
 def tree_workspace_bytes(num_tokens: int, num_seqs: int, max_q_len: int, H: int, H_kv: int,
                          D: int, block_size: int, max_blocks: int,
                          cache_dtype: torch.dtype = torch.bfloat16) -> int:

@@ -157,6 +157,26 @@ void heads_contiguous(T t, const char* text) {
   if (t->stride(2) != 1 || t->stride(1) != t->size(2)) value_error(text);
 }
 
+// Rows in memory: n of `bytes` bytes, `stride` bytes (at least that many) from one to the next.
+struct Rows {
+  const char* at;
+  int64_t n, bytes, stride;
+};
+
+// Whether two sets of rows share a byte. Rows that lie between each other's do not.
+bool meet(const Rows& a, const Rows& b) {
+  auto row = [](const Rows& r, int64_t i) { return r.at + i * r.stride; };
+  if (a.n == 0 || b.n == 0 || a.bytes == 0 || b.bytes == 0 || row(a, a.n - 1) + a.bytes <= b.at ||
+      row(b, b.n - 1) + b.bytes <= a.at)
+    return false;
+  for (int64_t i = 0, j = 0; i < a.n && j < b.n;) {
+    if (row(a, i) + a.bytes <= row(b, j)) ++i;
+    else if (row(b, j) + b.bytes <= row(a, i)) ++j;
+    else return true;
+  }
+  return false;
+}
+
 template <typename F> PyObject* guarded(F&& f) {
   HANDLE_TH_ERRORS
   try {
@@ -434,6 +454,11 @@ PyObject* logits(PyObject*, PyObject* const* a, Py_ssize_t) {
       if (out.dim() != 2 || out.size(0) != B || out.size(1) != V || out.scalar_type() != x->scalar_type() ||
           out.stride(1) != 1 || (B > 1 && out.stride(0) < V))
         value_error("out must be [B, V] of the logits' dtype with unit column stride");
+      const int64_t esz = x->element_size(), out_ld = std::max(out.stride(0), V);
+      const Rows from = {static_cast<const char*>(x->data_ptr()), B, V * esz, ld(x) * esz},
+                 to = {static_cast<const char*>(out.data_ptr()), B, V * esz, out_ld * esz};
+      if ((from.at != to.at || from.stride != to.stride) && meet(from, to))
+        value_error("out must be the logits themselves or not overlap them");
     }
     if (B > 0)
       call(lk_process_logits, out.data_ptr(), std::max(out.stride(0), V), ptr(x), n32(B), n32(V),

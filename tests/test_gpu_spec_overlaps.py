@@ -1,0 +1,36 @@
+"""Outputs that overlap an input, or each other, other than as documented are refused;
+those that lie beside or between each other's rows are not."""
+
+import pytest
+import torch
+
+from litevllm_b200 import ops
+
+pytestmark = pytest.mark.gpu
+
+BF16 = torch.bfloat16
+
+
+def test_process_logits(cuda):
+    V = 100
+    x = torch.randn((6, V), device=cuda)
+    freq, ids = torch.ones(4, device=cuda), torch.tensor([[3, 3, 7]] * 4, device=cuda)
+    call = lambda a, b: ops.process_logits(a, output_ids=ids, frequency=freq, out=b)  # noqa: E731
+    flat = x.flatten()
+    wide = torch.randn((4, 3 * V), device=cuda)
+    before, wide_before = x.clone(), wide.clone()
+    for a, b in ((x[:4], x[2:]), (x[1:5], x[:4]), (flat[:4 * V].view(4, V), flat[1:4 * V + 1].view(4, V)),
+                 (wide[:, :V], wide[:, V - 1:2 * V - 1]), (wide[:, V:2 * V], wide[:, :V + 1][:, 1:]),
+                 (wide[:, :V], wide.flatten()[:4 * V].view(4, V)),
+                 (wide.flatten()[:4 * V].view(4, V), wide[:, :V])):
+        with pytest.raises(ValueError, match="overlap"):
+            call(a, b)
+    torch.cuda.synchronize()
+    assert torch.equal(x, before) and torch.equal(wide, wide_before)
+    # beside, between and in place
+    for a, b in ((wide[:, :V], wide[:, V:2 * V]), (wide[:, 2 * V:], wide[:, :V]), (wide[::1, V:2 * V], wide[:, 2 * V:])):
+        want = call(a.clone(), None)
+        assert torch.equal(call(a, b), want)
+    even, odd = torch.randn((8, V), device=cuda).view(4, 2, V).unbind(1)
+    want = call(even.clone(), None)
+    assert torch.equal(call(even, odd), want) and torch.equal(call(even, even), want)

@@ -249,8 +249,11 @@ PyObject* load(PyObject*, PyObject* const* a, Py_ssize_t) {
           value_error("key_out/value_out must be contiguous [num_rows, H_kv, D] of dtype");
       }
     }
-    if (ko && vo && rows > 0 && ko->data_ptr() == vo->data_ptr())
-      value_error("key_out and value_out must be different tensors");
+    auto whole = [](const at::Tensor& t) {
+      return Rows{static_cast<const char*>(t.data_ptr()), 1, static_cast<int64_t>(t.nbytes()), 0};
+    };
+    if (meet(whole(outs[0]), whole(outs[1])))
+      value_error("key_out and value_out must be different tensors that do not overlap");
     call(lk_load_kv_q8, outs[0].data_ptr(), outs[1].data_ptr(), ptr(c.kd), ptr<float>(c.ks),
          ptr(c.vd), ptr<float>(c.vs), ptr<int32_t>(bt), bt->stride(0), ptr<int32_t>(ctx),
          ptr<int32_t>(cu), n32(B), rows, n32(c.H_kv), n32(c.D), c.nb, n32(c.bs), n32(max_blocks),

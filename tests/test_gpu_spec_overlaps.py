@@ -34,3 +34,20 @@ def test_process_logits(cuda):
     even, odd = torch.randn((8, V), device=cuda).view(4, 2, V).unbind(1)
     want = call(even.clone(), None)
     assert torch.equal(call(even, odd), want) and torch.equal(call(even, even), want)
+
+
+def test_load(cuda):
+    k, v = (ops.new_quantized_cache(2, 16, 2, 64, device=cuda) for _ in range(2))
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device=cuda)  # noqa: E731
+    call = lambda a, b: ops.load_kvcache_q8(k, v, i32([0, 1]), i32(20), i32(0, 20), 20, key_out=a, value_out=b)  # noqa: E731
+    both = torch.full((40, 2, 64), 3.0, dtype=BF16, device=cuda)
+    for lo in (0, 1, 19):
+        for a, b in ((both[lo:lo + 20], both[:20]), (both[:20], both[lo:lo + 20])):
+            with pytest.raises(ValueError, match="overlap"):
+                call(a, b)
+    torch.cuda.synchronize()
+    assert (both == 3).all()
+    call(both[20:], both[:20])
+    assert (both == 0).all()
+    none = both[:0]
+    ops.load_kvcache_q8(k, v, i32([0, 1]), i32(20), i32(0, 0), 0, key_out=none, value_out=none)

@@ -326,7 +326,8 @@ int lk_paged_prefill_ws(void* out, const void* q, int64_t q_token_stride,
  * 128, any block_size, any G = H / H_kv; caches 16-byte aligned. Scores,
  * softmax and sums are fp32; weights are rounded to 16 bits before the product
  * with V (f16 for 8-bit caches, the cache's type otherwise).
- * Rows of out that belong to no sequence are left as they were. *status (may
+ * Rows of out that belong to no sequence are left as they were; out may be q
+ * (with its stride), and otherwise must not overlap it. *status (may
  * be NULL) receives LK_STATUS_BLOCK_OOB (a block id outside the cache: that key's
  * row reads zeros) and LK_STATUS_CTX_OOB (a context longer than the table or
  * shorter than n, or a cu_seqlens_q that passes num_tokens or max_q_len).

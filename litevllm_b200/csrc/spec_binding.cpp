@@ -157,7 +157,7 @@ void heads_contiguous(T t, const char* text) {
   if (t->stride(2) != 1 || t->stride(1) != t->size(2)) value_error(text);
 }
 
-// Rows in memory: n of `bytes` bytes, `stride` bytes (at least that many) from one to the next.
+// Rows in memory: n of `bytes` bytes, `stride` bytes from one to the next.
 struct Rows {
   const char* at;
   int64_t n, bytes, stride;
@@ -355,6 +355,11 @@ PyObject* tree(PyObject*, PyObject* const* a, Py_ssize_t) {
       if (out.dim() != 3 || out.sizes() != query->sizes() || out.scalar_type() != query->scalar_type() ||
           out.stride(2) != 1 || out.stride(1) != D || (n > 1 && out.stride(0) < H * D))
         value_error("bad out tensor");
+      const int64_t esz = query->element_size();
+      const Rows from = {static_cast<const char*>(query->data_ptr()), n, H * D * esz, query->stride(0) * esz},
+                 to = {static_cast<const char*>(out.data_ptr()), n, H * D * esz, out.stride(0) * esz};
+      if ((from.at != to.at || (n > 1 && from.stride != to.stride)) && meet(from, to))
+        value_error("out must be the query itself or not overlap it");
     }
     auto result = [&]() { return out_in ? Py_NewRef(a[9]) : THPVariable_Wrap(out); };
     if (n == 0 || B == 0 || max_q == 0) return result();

@@ -190,11 +190,20 @@ def spec_module():
             f"{SPEC_PATH} is missing: build it with `python -m litevllm_b200.build`; "
             "there is no fallback implementation"
         )
-    import torch  # noqa: F401  (its libraries, which the binding links to)
+    import torch  # its libraries, which the binding links to
 
     spec = importlib.util.spec_from_file_location("litevllm_b200._spec", SPEC_PATH)
-    module = importlib.util.module_from_spec(spec)
-    spec.loader.exec_module(module)
+    try:
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+        built_for = getattr(module, "torch_version", "another version")
+    except ImportError as e:  # symbols of another torch
+        built_for, module = str(e), None
+    if module is None or built_for != torch.__version__:
+        raise LiteKernError(
+            f"{SPEC_PATH} does not fit torch {torch.__version__} ({built_for}): build it with "
+            "`python -m litevllm_b200.build`"
+        )
     return module
 
 

@@ -86,29 +86,37 @@ def build(force: bool = False, verbose: bool = False) -> Path:
 
 
 def build_spec(force: bool = False, verbose: bool = False) -> Path:
-    """The binding, with g++ against the installed torch; liblitekern.so comes first."""
+    """The binding, with g++ against the installed torch; liblitekern.so comes first.
+    It is built again when its sources, torch, Python or the command change: the
+    file beside the objects holds what the last one was built with."""
     import torch
 
     src = CSRC / "spec_binding.cpp"
-    newest = max(p.stat().st_mtime for p in [src, *INCLUDE.glob("*.h")])
-    if not force and SPEC.exists() and SPEC.stat().st_mtime >= newest:
-        return SPEC
     troot = Path(torch.__file__).resolve().parent
     cuda = Path(nvcc()).resolve().parent.parent
     tmp = SPEC.with_suffix(".so.tmp")
     cmd = [
         os.environ.get("CXX", "g++"), "-std=c++17", "-O2", "-fPIC", "-shared", f"-I{INCLUDE}",
+        f'-DLK_TORCH_VERSION="{torch.__version__}"',
         f"-I{troot}/include", f"-I{troot}/include/torch/csrc/api/include", f"-I{cuda}/include",
         f"-I{sysconfig.get_paths()['include']}", str(src), "-o", str(tmp), f"-L{PKG}",
         "-l:liblitekern.so", f"-L{troot}/lib", "-ltorch_python", "-ltorch_cpu", "-lc10_cuda", "-lc10",
         "-Wl,-rpath,$ORIGIN",
     ]
+    built_with = BUILD / "_spec.txt"
+    key = "\n".join([sys.version, sysconfig.get_config_var("SOABI"), *cmd])
+    newest = max(p.stat().st_mtime for p in [src, *INCLUDE.glob("*.h")])
+    if (not force and SPEC.exists() and SPEC.stat().st_mtime >= newest and built_with.exists()
+            and built_with.read_text() == key):
+        return SPEC
     if verbose:
         print(" ".join(cmd), flush=True)
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         raise RuntimeError(f"g++ failed on {src.name}:\n{res.stdout}\n{res.stderr}")
     os.replace(tmp, SPEC)
+    BUILD.mkdir(exist_ok=True)
+    built_with.write_text(key)
     return SPEC
 
 

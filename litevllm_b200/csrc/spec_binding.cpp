@@ -509,4 +509,9 @@ PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_spec", nullptr, -1, g_methods};
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__spec() { return PyModule_Create(&g_module); }
+PyMODINIT_FUNC PyInit__spec() {
+  PyObject* m = PyModule_Create(&g_module);
+  // the loader compares it with the torch it is loaded beside
+  if (m && PyModule_AddStringConstant(m, "torch_version", LK_TORCH_VERSION) < 0) Py_CLEAR(m);
+  return m;
+}

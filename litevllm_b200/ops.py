@@ -293,7 +293,8 @@ def tree_mask_from_parents(parents, device=None) -> torch.Tensor:
     for bits in rows:
         w = [(bits >> (64 * k)) & (2**64 - 1) for k in range(words)]
         out.append([x - 2**64 if x >> 63 else x for x in w])
-    return torch.tensor(out, dtype=torch.int64).view(len(rows), words).to(device or "cpu")
+    return torch.tensor(out, dtype=torch.int64, device="cpu" if device is None else device).view(
+        len(rows), words)
 
 
 # ----------------------------------------------------------- paged decode ---

@@ -142,3 +142,13 @@ def test_rows_of_scale_zero_outweigh_far_smaller_scores(cuda, kind, counts):
     got = run(c, cuda)
     check(c, got)
     assert (got == 0).all()
+
+
+def test_mask_on_a_device_given_by_its_number(cuda):
+    from litevllm_b200 import ops
+
+    for device in (0, "cuda", cuda):
+        m = ops.tree_mask_from_parents([[-1, 0, 0]], device)
+        assert m.device == cuda and m.flatten().tolist() == [1, 3, 5]
+        assert ops.tree_mask_from_parents([], device).device == cuda
+    assert ops.tree_mask_from_parents([[-1]]).device.type == "cpu"

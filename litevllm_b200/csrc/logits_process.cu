@@ -310,11 +310,8 @@ int launch_logits(const LogitsParams& p, int B, cudaStream_t s) {
   const bool vec =
       ((reinterpret_cast<uintptr_t>(p.logits) ^ reinterpret_cast<uintptr_t>(p.out)) & 15u) == 0 &&
       (((p.ld - p.out_ld) * static_cast<int64_t>(sizeof(T))) & 15) == 0;
+  static_assert(CH * 4 + kLList * 2 + kLMaxBias * 8 <= 48 * 1024, "no launch asks for more than the default");
   auto go = [&](auto* kernel) -> int {
-    if (smem > 48 * 1024 &&
-        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             static_cast<int>(smem)) != cudaSuccess)
-      return LK_ERR_CUDA;
     kernel<<<dim3(parts, B), kLThreads, smem, s>>>(p);
     return lk::check_launch();
   };

@@ -108,8 +108,8 @@ int lk_store_kv_q8(const void* key, const void* value, void* k_data, float* k_sc
 /*
  * Read an 8-bit cache back: row cu_rows[b] + p of key_out / value_out
  * ([num_rows, H_kv, D] contiguous, F32, F16 or BF16, 16-byte aligned) is
- * scale * q of position p of sequence b, rounded once, for
- * p < context_lens[b], and zero for the sequence's rows past its context.
+ * scale * q of position p of sequence b, the fp32 product rounded to the type,
+ * for p < context_lens[b], and zero for the sequence's rows past its context.
  * cu_rows: int32 [num_seqs + 1], not decreasing; rows before cu_rows[0] or
  * from cu_rows[num_seqs] on are left as they were. A context longer than the
  * table is flagged LK_STATUS_CTX_OOB and its rows past the table are zero; a

@@ -17,9 +17,13 @@
 // part in shared memory (so no [B, V] count tensor exists) and lists them, and
 // computes those few tokens, and the biased ones, again from their logits, while
 // other CTAs of the SM are in their dense pass. 128 x 151936 bf16 with 16 biases,
-// masks and histories of up to 1024 + 512 tokens: 24 us (81 MB, 3.4 TB/s; a bare
-// copy 11); with the counts read for every vector it took 40. 8 rows of 128256
+// histories of up to 1024 + 512 tokens and every fourth row under a mask that
+// closes most of it (72 MB: closed vectors are not read): 24 us (3.0 TB/s; a bare
+// copy 11); with the counts read for every vector it took 40. Every part looks
+// through its row's whole history: 8192 + 2048 tokens take 62 us. 8 rows of 128256
 // fp32: 4.9 us, a launch and one CTA's chain of dependent steps.
+// Seven CTAs per SM leave 32 registers: the aligned forms spill 84 to 148 bytes, which
+// the batch gains more than it costs; a few rows would not need so many CTAs.
 // Rows whose addresses are not multiples of 16 bytes keep 16-byte accesses:
 // tokens are indexed from the aligned address in front of the row.
 #include "lk_common.cuh"

@@ -110,7 +110,8 @@ struct Plan {
 //    (32 x 1000, 24 rows: 16-bit 27 and 33 on mma.sync, int8 32 and 35; 16 rows: 27 and
 //    28, 32 and 25) and the whole call outweighs its longer set-up (1 x 4000, 128 rows:
 //    16 and 28; 8 x 512, 64 rows: 16 and 14; 1 x 256, 256 rows: 12 and 9). Its TMA boxes
-//    want block sizes that are multiples of 16.
+//    want block sizes that are multiples of 16: with others wide trees stay on mma.sync
+//    (16 x 1K-8K, 192-256 rows, int8: blocks of 24 441 us, of 16 200).
 //  * Else NT, the smallest of 1, 2, 4 whose 8 NT rows hold a KV head's, or a smaller
 //    one while its units still leave room on the SMs: a warp with fewer accumulators
 //    is faster, and re-reads come from L2 (16 rows, 8 x 1000: NT 1 13.3, NT 2 13.8;

@@ -115,10 +115,10 @@ def _prefill(query, key_cache, value_cache, cu_seqlens_q, max_q_len, scale, bloc
     each = 2 * blocks * key_cache.data[0].numel() * query.element_size()
     step = max(1, Q8_PREFILL_BYTES // each)
     for b in range(0, S, step):
-        some = slice(b, b + step)
+        some = slice(b, min(b + step, S))
         k, v, tables = ops.load_kvcache_q8_blocks(key_cache, value_cache, block_tables[some],
                                                   context_lens[some], dtype=query.dtype)
-        ops.paged_prefill(query, k, v, cu_seqlens_q[b:b + step + 1], max_q_len, scale,
+        ops.paged_prefill(query, k, v, cu_seqlens_q[b:some.stop + 1], max_q_len, scale,
                           block_tables=tables, context_lens=context_lens[some], out=out)
         del k, v, tables  # before the next ones are allotted
     return out
@@ -301,7 +301,8 @@ class Attention(nn.Module):
         def prefill():
             _prefill(
                 query[:TP], key_cache, value_cache, cu_seqlens_q[: P + 1], max_q_len, self.scale,
-                block_tables=block_table[:P, :max_prefill_blocks], context_lens=context_lens[:P], out=out[:TP],
+                block_tables=block_table[:P, :max_prefill_blocks], context_lens=context_lens[:P],
+                out=out[:TP],
             )
 
         def decode():

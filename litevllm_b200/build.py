@@ -104,7 +104,7 @@ def build_spec(force: bool = False, verbose: bool = False) -> Path:
         "-Wl,-rpath,$ORIGIN",
     ]
     built_with = BUILD / "_spec.txt"
-    key = "\n".join([sys.version, sysconfig.get_config_var("SOABI"), *cmd])
+    key = "\n".join([sys.version, str(sysconfig.get_config_var("SOABI")), *cmd])
     newest = max(p.stat().st_mtime for p in [src, *INCLUDE.glob("*.h")])
     if (not force and SPEC.exists() and SPEC.stat().st_mtime >= newest and built_with.exists()
             and built_with.read_text() == key):

@@ -24,13 +24,14 @@
 // 900 S, 1500 the softmax, 900 P V, and two stages in each of two CTAs overlap them to
 // 2300 (16 bits) and 3200 cycles a chunk (8). 32 trees of 20-32 nodes over 64-2048
 // tokens, bf16, G = 4: 47 us (151 MB, 3.2 TB/s), the 32 chunks of the longest trees one
-// after the other, as one wave of CTAs leaves no room to cut them. 16 trees of 48-64 over 1K-8K, int8:
-// 200 us (337 TFLOP/s). The loop is half of that: 62 chunks a resident CTA are 100 us,
-// pieces of unequal length in the order of their start and 4 us of set-up each make it
-// 128, the join is 17, and what the other 50 go to is not known (the tensor pipe is 22 % busy over all,
-// 46 % would go with 3200 cycles a chunk throughout). With the bytes of one chunk of K
-// at a time in a buffer of their own the int8 case took 254, with suspending waits for the
-// copies 230, with one thread alone in the MMA warp's loop 212.
+// after the other, as one wave of CTAs leaves no room to cut them. 16 trees of 48-64
+// over 1K-8K, int8: 200 us (337 TFLOP/s). The loop is half of that: 62 chunks a resident
+// CTA are 100 us, pieces of unequal length in the order of their start and 4 us of set-up
+// each make it 128, the join is 17, and what the other 50 go to is not known (the tensor
+// pipe is 22 % busy over all, 46 % would go with 3200 cycles a chunk throughout). With
+// the bytes of one chunk of K at a time in a buffer of their own the int8 case took 254,
+// with suspending waits for the copies 230, with one thread alone in the MMA warp's
+// loop 212.
 // The weights are rounded to the operand type for P V, as the tensor core takes it (the
 // denominator sums them before): f16, 11 bits, over 8-bit caches; over a bf16 cache 8
 // bits, each weight off by up to 2^-8 of itself, as in the other attention kernels here.
